@@ -78,6 +78,16 @@ def _stream() -> int:
     return _PINNED_STREAM[0] or torch.cuda.current_stream().cuda_stream
 
 
+def _device_stream(*tensors) -> int:
+    """The stream to launch on for tensors that all lie on the current device (a kernel of one device cannot be launched on another's
+    stream); anything else is refused."""
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+    return _PINNED_STREAM[0] or torch._C._cuda_getCurrentRawStream(here)
+
+
 class pin_stream:
     """``with pin_stream():`` every launch inside goes to the stream that is current on entry.  Code that
     switches streams inside (the weight prefetcher's side stream) passes its stream explicitly."""
@@ -2268,6 +2278,148 @@ class CudaKernels:
         _check(fn(_cuda(tokens, "tokens", torch.int32), _cuda(rows, "rows", torch.int32), _cuda(table, "expert table", torch.int32),
                   table.shape[0], num_experts, top, _cuda(ids, "expert ids", torch.int32), _cuda(weights, "expert weights", torch.float32),
                   weight, n, tokens.numel(), _stream()), "moe_table_route")
+
+    # ---- which experts a token takes where experts come in groups (csrc/moe_groups.cu) -----------------------------------------
+    def moe_route_grouped(self, logits: torch.Tensor, top: int, ids: torch.Tensor, weights: torch.Tensor, *, score: str = "sigmoid",
+                          correction: Optional[torch.Tensor] = None, groups: int = 1, top_groups: int = 1, group_top: int = 2,
+                          renormalise: bool = True, scale: float = 1.0) -> None:
+        """Router logits (float32 [N, E], may be a column slice) -> the ``top`` experts of each token and their weights.
+
+        ``s`` = ``score`` (``sigmoid`` or ``softmax`` over all E) of the logits, ``c = s + correction``.  A group is ``E / groups`` neighbouring
+        experts, its score the sum of its ``group_top`` (1 or 2) largest ``c``.  Of the ``top_groups`` groups with the largest scores the
+        ``top`` experts with the largest ``c`` are taken, largest first; ties go to the lower index, and scores are compared in 64 bits.  An
+        expert weighs ``scale * s``, with ``renormalise`` divided by the sum of the chosen ``s`` (0 where that is 0).  E up to 1,024, up to
+        32 groups and 32 experts a token."""
+        n, e = logits.shape
+        if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top) or (correction is not None and correction.numel() != e):
+            raise KernelError("moe_route_grouped: logits float32 [N, E]; correction [E]; ids / weights [N, top]")
+        if score not in ("sigmoid", "softmax"):
+            raise KernelError(f"moe_route_grouped: score is 'sigmoid' or 'softmax', not {score!r}")
+        if groups < 1 or e % groups or not 1 <= top_groups <= groups or group_top not in (1, 2) or not 1 <= top <= top_groups * (e // groups):
+            raise KernelError(f"moe_route_grouped: {top} of {e} experts, {top_groups} of {groups} groups known by their best {group_top}")
+        lp, ld = self._rows(logits, "router logits")
+        stream = _device_stream(logits, ids, weights, correction)
+        if n == 0:
+            return
+        fn = _fn("moe_groups", "iian_moe_route_grouped", [c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                          c_float, c_void_p, c_void_p, c_int, c_void_p])
+        _check(fn(lp, ld, _cuda(correction, "choice correction", torch.float32), e, groups, top_groups, group_top, top, int(score == "softmax"),
+                  int(renormalise), scale, _cuda(ids, "expert ids", torch.int32), _cuda(weights, "expert weights", torch.float32), n, stream),
+               "moe_route_grouped")
+
+    # ---- products with what follows them in their epilogue (csrc/linear_fused.cu, csrc/gemm_simt.cu) ------------------------------
+    LINEAR_ACTIVATIONS = {"none": 0, "silu": 1, "gelu_tanh": 2, "gelu": 3, "relu": 4, "relu2": 5}
+
+    @staticmethod
+    def _product_rows(x: torch.Tensor, w: torch.Tensor, what: str):
+        """(pointer of x, row stride, whether the tensor cores' product takes x and w) for x [N, K] and w [M, K]."""
+        if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+            raise KernelError(f"{what}: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
+        if x.dtype not in _CODE or w.dtype not in _CODE:
+            raise KernelError(f"{what}: x and w are float32 or bfloat16")
+        n, k = x.shape
+        xp, ld = CudaKernels._rows(x, f"{what} x")
+        if n <= 1:
+            ld = k
+        if k < 1 or ld < k:
+            raise KernelError(f"{what}: rows of x overlap or are empty")
+        tc = (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and k % 8 == 0 and ld % 8 == 0 and xp % 16 == 0
+              and w.data_ptr() % 16 == 0)
+        return xp, ld, tc
+
+    def linear_act(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                   residual: Optional[torch.Tensor] = None, form: int = 0) -> None:
+        """``out = residual + act(x w^T + bias)``: float32 until the one rounding into ``out``.
+
+        x [N, K] and w [M, K] float32 or bfloat16, ``bias`` float32 [M], ``residual`` and ``out`` [N, M] float32 or bfloat16 each; rows of x,
+        residual and out may be apart.  ``residual`` may be ``out`` itself (the same tensor, or one of the same place, type and row distance);
+        other than that out overlaps none of them.  ``activation``: ``none``, ``silu``, ``gelu_tanh``, ``gelu`` (by erf), ``relu``, ``relu2``.  ``form``: a
+        tile of the tensor cores' product other than the one it chooses (csrc/linear_fused.cu)."""
+        xp, ldx, tc = self._product_rows(x, w, "linear_act")
+        (n, k), m = x.shape, w.shape[0]
+        act = self.LINEAR_ACTIVATIONS.get(activation)
+        if act is None:
+            raise KernelError(f"linear_act: activation {activation!r} has no kernel ({', '.join(self.LINEAR_ACTIVATIONS)})")
+        if out.shape != (n, m) or (bias is not None and bias.numel() != m) or (residual is not None and residual.shape != (n, m)):
+            raise KernelError(f"linear_act: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}, bias [M], residual [N, M] do not fit")
+        oc, op, ldo = _code(out, "linear_act out"), *self._rows(out, "linear_act out")
+        rc, rp, ldr = (_code(residual, "linear_act residual"), *self._rows(residual, "linear_act residual")) if residual is not None else (0, 0, 0)
+        if n > 1 and ldo < m:
+            raise KernelError("linear_act: rows of out overlap")
+        if rp and rp == op and (rc != oc or (n > 1 and ldr != ldo)):
+            raise KernelError("linear_act: a residual in the place of out has its type and row distance")
+        stream = _device_stream(x, w, out, bias, residual)
+        if n == 0 or m == 0:
+            return
+        wp, bp = _cuda(w, "linear_act w"), _cuda(bias, "linear_act bias", torch.float32)
+        if tc:
+            status = self.tcgen05_status_buffer(x.device).data_ptr()
+            CudaKernels._tc_used = True
+            fn = _fn("linear_fused", "iian_linear_act", [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int,
+                                                         c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+            _check(fn(xp, ldx, wp, bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, form, status, stream), "linear_act")
+            return
+        fn = _fn("gemm_simt", "iian_linear_act_simt", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
+                                                       c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p])
+        _check(fn(xp, _CODE[x.dtype], ldx, wp, _CODE[w.dtype], bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, stream), "linear_act_simt")
+
+    SCORE_ROWS = 16384          # rows of one launch: their partial sums take up to 8 bytes a row and 128 columns
+    SCORE_PIECE = 1 << 24       # logits that are in memory at a time where the tensor cores' product does not take the operands
+
+    def linear_logprobs(self, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, logprobs: torch.Tensor, lse: torch.Tensor,
+                        softcap: Optional[float] = None, form: int = 0) -> None:
+        """Log-probabilities of given tokens without the logits: with ``z = x w^T`` (and ``z = c tanh(z / c)`` where ``softcap`` is c),
+        ``lse[t] = log sum_v exp z[t, v]`` and ``logprobs[t] = z[t, targets[t]] - lse[t]``, all float32.
+
+        x [N, K] (rows may be apart) and w [V, K] float32 or bfloat16, targets int32 [N].  A negative target is none: its log-probability is
+        0; one of V or more gives what is no number.  A row of nothing but minus infinity has the log-sum-exp minus infinity.  The working
+        memory, a pair of floats a row and some 200 columns, is the call's own."""
+        xp, ldx, tc = self._product_rows(x, w, "linear_logprobs")
+        (n, k), v = x.shape, w.shape[0]
+        if targets.shape != (n,) or logprobs.shape != (n,) or lse.shape != (n,) or v < 1:
+            raise KernelError(f"linear_logprobs: x {tuple(x.shape)}, w {tuple(w.shape)}; targets, logprobs and lse [N] do not fit")
+        cap = float(softcap) if softcap is not None else 0.0
+        if not 0.0 <= cap < float("inf") or (softcap is not None and cap == 0.0):
+            raise KernelError("linear_logprobs: softcap must be positive")
+        tp, op, sp = (_cuda(targets, "linear_logprobs targets", torch.int32), _cuda(logprobs, "linear_logprobs out", torch.float32),
+                      _cuda(lse, "linear_logprobs lse", torch.float32))
+        if op == sp and n > 0:
+            raise KernelError("linear_logprobs: logprobs and lse are two tensors")
+        stream = _device_stream(x, w, targets, logprobs, lse)
+        wp, esize = _cuda(w, "linear_logprobs w"), x.element_size()
+        for r in range(0, n, self.SCORE_ROWS):
+            t = min(self.SCORE_ROWS, n - r)
+            at = (tp + 4 * r, op + 4 * r, sp + 4 * r)
+            if tc:
+                status = self.tcgen05_status_buffer(x.device).data_ptr()
+                CudaKernels._tc_used = True
+                tiles = _fn("linear_fused", "iian_linear_logprobs_tiles", [c_int, c_int, c_int])(t, v, form)
+                part = torch.empty(2 * max(1, tiles) * t, dtype=torch.float32, device=x.device)
+                fn = _fn("linear_fused", "iian_linear_logprobs", [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                                                  c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+                _check(fn(xp + r * ldx * esize, ldx, wp, *at, part.data_ptr(), t, v, k, cap, form, status, stream), "linear_logprobs")
+                LAUNCHES[0] += 1
+                continue
+            self._logprobs_pieces(x[r: r + t], xp + r * ldx * esize, ldx, w, wp, at, t, v, k, cap, stream)
+
+    def _logprobs_pieces(self, x, xp, ldx, w, wp, at, t, v, k, cap, stream) -> None:
+        """The same with the logits of a piece of the vocabulary at a time in memory, from the product that takes every type and size."""
+        width = min(v, max(4096, self.SCORE_PIECE // t))
+        splits = max(1, min(64, width // 2048, 1024 // t))
+        pieces = -(-v // width)
+        logits = torch.empty(t * width, dtype=torch.float32, device=x.device)
+        part = torch.empty(2 * pieces * splits * t, dtype=torch.float32, device=x.device)
+        product = _fn("gemm_simt", "iian_linear_act_simt", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
+                                                            c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p])
+        take = _fn("linear_fused", "iian_linear_logprobs_piece", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                                                  c_float, c_void_p])
+        for i in range(pieces):
+            v0, p = i * width, min(width, v - i * width)
+            _check(product(xp, _CODE[x.dtype], ldx, wp + v0 * k * w.element_size(), _CODE[w.dtype], 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k,
+                           0, stream), "linear_act_simt")
+            _check(take(logits.data_ptr(), t, p, v0, at[0], at[1], part.data_ptr(), i * splits, splits, cap, stream), "linear_logprobs_piece")
+        join = _fn("linear_fused", "iian_linear_logprobs_join", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+        _check(join(part.data_ptr(), pieces * splits, t, v, *at, stream), "linear_logprobs_join")
 
     # ---- sampling ------------------------------------------------------------------------
     def argmax(self, logits: torch.Tensor, out: torch.Tensor) -> None:
