@@ -6,14 +6,49 @@ namespace iian {
 
 enum { LACT_NONE = 0, LACT_SILU = 1, LACT_GELU_TANH = 2, LACT_GELU = 3, LACT_RELU = 4, LACT_RELU2 = 5, LACT_COUNT = 6 };
 
-__device__ __forceinline__ float linear_act_value(float y, int act) {
+// What bounds an epilogue with an activation is the hardware's exponential and reciprocal (8 cycles each for a warp), so each form has as few
+// of them as it can.  silu is y / (1 + e^-y), gelu_tanh y / (1 + e^-2u), which is 0.5 y (1 + tanh u) without the difference that loses
+// the digits of its lower tail.  gelu uses Abramowitz and Stegun's 7.1.28, erf x = 1 - (1 + a1 x + .. + a6 x^6)^-16, within 3e-7:
+// gelu y = max(y, 0) - |y| / 2 * that power, with one reciprocal and no exponential (7.1.26, which has both, took 4.3 us for the 128 x 256
+// outputs of a tile).  Results are float32 within a few 1e-7 of the value.
+__device__ __forceinline__ float linear_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float linear_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int ACT> __device__ __forceinline__ float linear_act_of(float y) {
+    if constexpr (ACT == LACT_SILU) return y * linear_rcp(1.0f + linear_exp2(-1.4426950408889634f * y));
+    else if constexpr (ACT == LACT_GELU_TANH)              // 2 sqrt(2 / pi) log2 e and 0.044715 times that
+        return y * linear_rcp(1.0f + linear_exp2(y * fmaf(y * y, -0.10294324f, -2.3022082f)));
+    else if constexpr (ACT == LACT_GELU) {
+        const float x = 0.7071067811865476f * fabsf(y);
+        float d = fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, 0.0000430638f, 0.0002765672f), 0.0001520143f), 0.0092705272f), 0.0422820123f), 0.0705230784f), 1.0f);
+        d *= d; d *= d; d *= d;
+        return fmaf(-0.5f * fabsf(y), linear_rcp(d * d), y < 0.0f ? 0.0f : y);
+    } else if constexpr (ACT == LACT_RELU) return y < 0.0f ? 0.0f : y;        // (what is no number stays none)
+    else if constexpr (ACT == LACT_RELU2) return y < 0.0f ? 0.0f : y * y;
+    else return y;
+}
+
+// One decision for all of COUNT values: between them the compiler interleaves, where each had its own branch they came one after the other
+// (2,048 x 12,288 x 4,096 with gelu 364 us).
+template <int COUNT> __device__ __forceinline__ void linear_act_values(float * y, int act) {
+    auto all = [&](auto one) {
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) y[i] = one(y[i]);
+    };
     switch (act) {
-        case LACT_SILU: return y / (1.0f + expf(-y));
-        case LACT_GELU_TANH: return 0.5f * y * (1.0f + tanhf(0.7978845608028654f * (y + 0.044715f * y * y * y)));
-        case LACT_GELU: return 0.5f * y * (1.0f + erff(0.7071067811865476f * y));
-        case LACT_RELU: return y < 0.0f ? 0.0f : y;          // (what is no number stays none)
-        case LACT_RELU2: return y < 0.0f ? 0.0f : y * y;
-        default: return y;
+        case LACT_SILU: all([](float v) { return linear_act_of<LACT_SILU>(v); }); break;
+        case LACT_GELU_TANH: all([](float v) { return linear_act_of<LACT_GELU_TANH>(v); }); break;
+        case LACT_GELU: all([](float v) { return linear_act_of<LACT_GELU>(v); }); break;
+        case LACT_RELU: all([](float v) { return linear_act_of<LACT_RELU>(v); }); break;
+        case LACT_RELU2: all([](float v) { return linear_act_of<LACT_RELU2>(v); }); break;
+        default: break;
     }
 }
 
@@ -25,88 +60,64 @@ struct LinearEpilogue {
     void * out;
     long long ldr, ldo;
     int act, res_bf16, out_bf16;
-    int res_vec, out_vec, bias_vec;       // whether 8 neighbouring columns from a multiple of 8 on lie on 16 bytes
+    int res_vec, out_vec, bias_vec;       // whether 4 neighbouring columns from a multiple of 4 on are one aligned access
 
-    __device__ __forceinline__ float one(float y, size_t row, int col) const {
-        if (bias != nullptr) y += bias[col];
-        y = linear_act_value(y, act);
-        if (res != nullptr) {
-            const size_t at = row * (size_t) ldr + col;
-            y += res_bf16 ? __bfloat162float(((const __nv_bfloat16 *) res)[at]) : ((const float *) res)[at];
-        }
-        return y;
+    __device__ __forceinline__ float residual1(size_t at) const {
+        return res_bf16 ? __bfloat162float(((const __nv_bfloat16 *) res)[at]) : ((const float *) res)[at];
     }
-    __device__ __forceinline__ void store(float y, size_t row, int col) const {
-        y = one(y, row, col);
-        const size_t at = row * (size_t) ldo + col;
+    __device__ __forceinline__ void put1(float y, size_t at) const {
         if (out_bf16) ((__nv_bfloat16 *) out)[at] = __float2bfloat16_rn(y);
         else ((float *) out)[at] = y;
     }
-    // 8 columns from col on, `live` of them inside the matrix
-    __device__ __forceinline__ void store8(float * y, size_t row, int col, int live) const {
-        if (live < 8) {
-#pragma unroll
-            for (int i = 0; i < 7; i++)
-                if (i < live) store(y[i], row, col + i);
+    __device__ __forceinline__ void store(float y, size_t row, int col) const {
+        if (bias != nullptr) y += bias[col];
+        linear_act_values<1>(&y, act);
+        if (res != nullptr) y += residual1(row * (size_t) ldr + col);
+        put1(y, row * (size_t) ldo + col);
+    }
+    // 4 columns from col (a multiple of 4) on, `live` of them inside the matrix: the bias, the residual, and the results
+    __device__ __forceinline__ float4 bias4(int col, int live) const {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (bias == nullptr || live <= 0) return v;
+        if (live >= 4 && bias_vec) return __ldg(reinterpret_cast<const float4 *>(bias + col));
+        v.x = bias[col];
+        if (live > 1) v.y = bias[col + 1];
+        if (live > 2) v.z = bias[col + 2];
+        if (live > 3) v.w = bias[col + 3];
+        return v;
+    }
+    __device__ __forceinline__ float4 residual4(size_t row, int col, int live) const {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (res == nullptr || live <= 0) return v;
+        const size_t at = row * (size_t) ldr + col;
+        if (live >= 4 && res_vec) {
+            if (!res_bf16) return *reinterpret_cast<const float4 *>((const float *) res + at);
+            const uint2 raw = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *) res + at);
+            const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.y));
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+        v.x = residual1(at);
+        if (live > 1) v.y = residual1(at + 1);
+        if (live > 2) v.z = residual1(at + 2);
+        if (live > 3) v.w = residual1(at + 3);
+        return v;
+    }
+    __device__ __forceinline__ void put4(const float * y, size_t row, int col, int live) const {
+        if (live <= 0) return;
+        const size_t at = row * (size_t) ldo + col;
+        if (live >= 4 && out_vec) {
+            if (out_bf16) {
+                __nv_bfloat162 p[2] = {__floats2bfloat162_rn(y[0], y[1]), __floats2bfloat162_rn(y[2], y[3])};
+                *reinterpret_cast<uint2 *>((__nv_bfloat16 *) out + at) = *reinterpret_cast<uint2 *>(p);
+            } else {
+                *reinterpret_cast<float4 *>((float *) out + at) = make_float4(y[0], y[1], y[2], y[3]);
+            }
             return;
         }
-        if (bias != nullptr) {
-            if (bias_vec) {
-                const float4 a = __ldg(reinterpret_cast<const float4 *>(bias + col)), b = __ldg(reinterpret_cast<const float4 *>(bias + col + 4));
-                y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w; y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] += bias[col + i];
-            }
-        }
-        if (act != LACT_NONE) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = linear_act_value(y[i], act);
-        }
-        if (res != nullptr) {
-            const size_t at = row * (size_t) ldr + col;
-            if (res_bf16) {
-                const __nv_bfloat16 * r = (const __nv_bfloat16 *) res + at;
-                float f[8];
-                if (res_vec) unpack8(*reinterpret_cast<const uint4 *>(r), f);
-                else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) f[i] = __bfloat162float(r[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] += f[i];
-            } else {
-                const float * r = (const float *) res + at;
-                if (res_vec) {
-                    const float4 a = *reinterpret_cast<const float4 *>(r), b = *reinterpret_cast<const float4 *>(r + 4);
-                    y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w; y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] += r[i];
-                }
-            }
-        }
-        const size_t at = row * (size_t) ldo + col;
-        if (out_bf16) {
-            __nv_bfloat16 * o = (__nv_bfloat16 *) out + at;
-            __nv_bfloat162 p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-            if (out_vec) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<uint4 *>(p);
-            else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) { o[2 * i] = p[i].x; o[2 * i + 1] = p[i].y; }
-            }
-        } else {
-            float * o = (float *) out + at;
-            if (out_vec) {
-                *reinterpret_cast<float4 *>(o) = make_float4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<float4 *>(o + 4) = make_float4(y[4], y[5], y[6], y[7]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) o[i] = y[i];
-            }
-        }
+        put1(y[0], at);
+        if (live > 1) put1(y[1], at + 1);
+        if (live > 2) put1(y[2], at + 2);
+        if (live > 3) put1(y[3], at + 3);
     }
 };
 
@@ -118,8 +129,8 @@ static inline bool linear_epilogue(LinearEpilogue & e, const float * bias, const
     e.res_bf16 = res_dtype == IIAN_BF16;
     e.out_bf16 = out_dtype == IIAN_BF16;
     e.bias_vec = ((uintptr_t) bias & 15) == 0;
-    e.res_vec = ((uintptr_t) res & 15) == 0 && ldr * (e.res_bf16 ? 2 : 4) % 16 == 0;
-    e.out_vec = ((uintptr_t) out & 15) == 0 && ldo * (e.out_bf16 ? 2 : 4) % 16 == 0;
+    e.res_vec = (uintptr_t) res % (e.res_bf16 ? 8 : 16) == 0 && ldr % 4 == 0;
+    e.out_vec = (uintptr_t) out % (e.out_bf16 ? 8 : 16) == 0 && ldo % 4 == 0;
     return true;
 }
 

@@ -22,6 +22,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -29,18 +30,37 @@
 
 namespace iian {
 
-constexpr int LF_STAGES = 16;             // barriers there are; how many are used follows from the size of a stage
+constexpr int LF_STAGES = 24;             // barriers there are; how many are used follows from the size of a stage
+constexpr int LF_WARPS = 8;               // epilogue warps: two for each quarter of the accumulator's lanes, sharing its columns
+constexpr int LF_THREADS = 64 + 32 * LF_WARPS;
+constexpr int LF_COLS = 16;               // columns an epilogue warp turns around at a time; rows of 64 bytes, their 16-byte pieces swapped so that
+                                          // neither writing a row a lane nor reading two rows by eight lanes meets a bank twice
+constexpr int LF_TURN = 128 / LF_COLS, LF_TURNS = 32 / LF_TURN;       // rows a warp's access covers, and accesses for 32 rows
+constexpr int kLfRing = 208 * 1024, kLfSmem = kLfRing + LF_WARPS * 32 * LF_COLS * 4 + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LfScore {
-    float2 * part;                        // [column tiles][T]: maximum and sum of a row's columns in a tile
+    float2 * part;                        // [2 column tiles][T]: maximum and sum of a row's columns in a tile, of one warp's and of the other's
     const int * targets;
     float * lp;                           // receives the target's logit
     float cap;                            // 0: none
 };
 
+// What follows the product.  LF_ANY takes every type, place and width an entry at a time where it has to; the four others have their types fixed
+// and every access of 4 columns whole and aligned, so that nothing is decided between the sums and the store (2,048 x 4,096 outputs behind a
+// K of 64, which is all epilogue: 18 us with the decisions).
+enum { LF_SCORE = 0, LF_ANY = 1, LF_BF16 = 2, LF_F32 = 3, LF_BF16_RES = 4, LF_F32_RES = 5 };       // (the residual of the last two is float32)
+
 struct LfArgs {
-    int T, N, K, bn, ks, stages, a_rows, stage_bytes;
+    int T, N, bn, ks, stages, stage_bytes, a_bytes, kb_bytes, all_kb, m_tiles, num_tiles, units;
+    // where K is shared: a CTA adds up `per` of the tile's groups of 4 columns (inv_per = 65536 / per, rounded up); the parts arrive at
+    // recv_off, rows of recv_ld groups for every CTA that sends, over the ring (recv_shared) or behind it
+    int per, inv_per, recv_off, recv_ld, recv_rows, recv_shared;
+    // a tile's K blocks go to `accs` accumulators in turn, added up in the epilogue: the sums in tensor memory are not rounded but cut off, so
+    // that the error grows with the length of the chain, and products into one accumulator wait for one another (90 ns each however few
+    // columns they have); buf_cols: columns of all of them
+    int accs, buf_cols;
+    unsigned tmem_cols;
     TcStatus * status;
     LinearEpilogue epi;
     LfScore score;
@@ -55,6 +75,30 @@ __device__ __forceinline__ float lf_finite_or_zero(float m) { return fabsf(m) < 
 // c tanh(z / c) with the hardware's exponential: tanh's absolute error is a few 1e-7
 __device__ __forceinline__ float lf_cap_fast(float z, float cap, float two_over_cap_log2e) {
     return cap * (1.0f - __fdividef(2.0f, 1.0f + lf_exp2(z * two_over_cap_log2e)));
+}
+
+// LF_COLS columns of 32 lanes
+__device__ __forceinline__ void lf_ld(unsigned taddr, unsigned * r) {
+    static_assert(LF_COLS == 16, "");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+
+// the same of a tile's accumulators together, `between` columns apart
+__device__ __forceinline__ void lf_sum(unsigned taddr, int accs, int between, float * y) {
+    unsigned r[LF_COLS];
+    lf_ld(taddr, r);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < LF_COLS; i++) y[i] = __uint_as_float(r[i]);
+    for (int a = 1; a < accs; a++) {
+        lf_ld(taddr + (unsigned) (a * between), r);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < LF_COLS; i++) y[i] += __uint_as_float(r[i]);
+    }
 }
 
 // 32 columns of a row, `live` of them in the matrix, into the row's running maximum and sum
@@ -83,179 +127,239 @@ __device__ __forceinline__ unsigned lf_pick(const unsigned * r, int at) {
     return v;
 }
 
-template <bool PAIR, bool SCORE>
-__global__ void __launch_bounds__(TC_THREADS, 1) linear_fused_kernel(const __grid_constant__ CUtensorMap map_a,
+template <int KIND> __device__ __forceinline__ float4 lf_residual(const LinearEpilogue & e, size_t row, int col, int live) {
+    if constexpr (KIND == LF_ANY) return e.residual4(row, col, live);
+    else if constexpr (KIND == LF_BF16_RES || KIND == LF_F32_RES)
+        return live > 0 ? *reinterpret_cast<const float4 *>((const float *) e.res + row * (size_t) e.ldr + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    else return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+template <int KIND> __device__ __forceinline__ float4 lf_bias(const LinearEpilogue & e, int col, int live) {
+    if constexpr (KIND == LF_ANY) return e.bias4(col, live);
+    else return e.bias != nullptr && live > 0 ? __ldg(reinterpret_cast<const float4 *>(e.bias + col)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+template <int KIND> __device__ __forceinline__ void lf_put(const LinearEpilogue & e, const float * y, const float4 & r, size_t row, int col, int live) {
+    float v[4] = {y[0] + r.x, y[1] + r.y, y[2] + r.z, y[3] + r.w};
+    if constexpr (KIND == LF_ANY) e.put4(v, row, col, live);
+    else if (live > 0) {
+        const size_t at = row * (size_t) e.ldo + col;
+        if constexpr (KIND == LF_BF16 || KIND == LF_BF16_RES) {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+            *reinterpret_cast<uint2 *>((__nv_bfloat16 *) e.out + at) = *reinterpret_cast<uint2 *>(h);
+        } else *reinterpret_cast<float4 *>((float *) e.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+template <bool PAIR, int KIND>
+__global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b, const LfArgs p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = (unsigned char *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
+    constexpr bool SCORE = KIND == LF_SCORE;
     constexpr int KPS = PAIR ? 2 : 1;     // blocks of K a stage
     constexpr int ROWS = PAIR ? 2 * TC_BM : TC_BM;
     __shared__ __align__(8) unsigned long long full_bar[LF_STAGES], empty_bar[LF_STAGES], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_base_s;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int bn = p.bn, half = PAIR ? bn / 2 : bn, stages = p.stages;
+    const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;        // (uniform, and known to be)
+    const int bn = p.bn, half = PAIR ? bn / 2 : bn, stages = p.stages, m_tiles = p.m_tiles, num_tiles = p.num_tiles, units = p.units;
     const unsigned cluster_rank = PAIR || p.ks > 1 ? cluster_cta_rank() : 0u;
-    const unsigned rank = PAIR ? cluster_rank : 0u;                           // which CTA of a pair
-    const int group = PAIR ? 2 : p.ks, unit = (int) blockIdx.x / group, units = (int) gridDim.x / group;
-    const int a_bytes = p.a_rows * TC_BK * 2, b_bytes = half * TC_BK * 2, kb_bytes = a_bytes + b_bytes;
-    const int blocks = (p.K + TC_BK - 1) / TC_BK, all_kb = (blocks + KPS - 1) / KPS;
-    const int kb0 = PAIR ? 0 : (int) ((long long) all_kb * cluster_rank / p.ks);
-    const int kb1 = PAIR ? all_kb : (int) ((long long) all_kb * (cluster_rank + 1) / p.ks);
-    const int m_tiles = (p.T + ROWS - 1) / ROWS, n_tiles = (p.N + bn - 1) / bn;
-    const long long num_tiles = (long long) m_tiles * n_tiles;
+    const unsigned rank = PAIR ? cluster_rank & 1u : 0u, leader = PAIR ? cluster_rank & ~1u : 0u;       // which CTA of a pair, and its first
+    const int split = (int) (PAIR ? cluster_rank >> 1 : cluster_rank);        // which share of K
+    const int block = PAIR ? (int) blockIdx.x >> 1 : (int) blockIdx.x, unit = p.ks > 1 ? block / p.ks : block;
+    const int a_bytes = p.a_bytes, kb_bytes = p.kb_bytes;
+    const int kb0 = p.ks > 1 ? p.all_kb * split / p.ks : 0, kb1 = p.ks > 1 ? p.all_kb * (split + 1) / p.ks : p.all_kb;
     const int acc_cols = (bn + 31) & ~31;
-    unsigned tmem_cols = 64;
-    while (tmem_cols < 2u * acc_cols) tmem_cols *= 2;
+    const int early = PAIR || unit >= num_tiles ? 0 : min(stages, kb1 - kb0);  // copies that are asked for before anything else is set up
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; s++) { mbar_init(smem_addr(&full_bar[s]), 1); mbar_init(smem_addr(&empty_bar[s]), 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&acc_full[b]), 1); mbar_init(smem_addr(&acc_empty[b]), PAIR ? 8 : 4); }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    auto copy = [&](int s, int kb, int m0, int n0) {
+        const unsigned to = smem_addr(smem + s * p.stage_bytes);
+        if constexpr (PAIR) {
+            const unsigned bar = map_to_cta(smem_addr(&full_bar[s]), leader);
+            if (rank == 0) mbar_expect_tx_warp(smem_addr(&full_bar[s]), 2 * KPS * kb_bytes);
+#pragma unroll
+            for (int j = 0; j < KPS; j++) {
+                tma_load_2d_pair_warp(to + j * kb_bytes, &map_a, (kb * KPS + j) * TC_BK, m0, bar);
+                tma_load_2d_pair_warp(to + j * kb_bytes + a_bytes, &map_b, (kb * KPS + j) * TC_BK, n0, bar);
+            }
+        } else {
+            const unsigned bar = smem_addr(&full_bar[s]);
+            mbar_expect_tx_warp(bar, kb_bytes);
+            tma_load_2d_warp(to, &map_a, kb * TC_BK, m0, bar);
+            tma_load_2d_warp(to + a_bytes, &map_b, kb * TC_BK, n0, bar);
+        }
+    };
+
+    pdl_launch_dependents();
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < stages; s++) { mbar_init(smem_addr(&full_bar[s]), 1); mbar_init(smem_addr(&empty_bar[s]), 1); }
+            for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&acc_full[b]), 1); mbar_init(smem_addr(&acc_empty[b]), PAIR ? 2 * LF_WARPS : LF_WARPS); }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        pdl_wait();
+        for (int i = 0; i < early; i++) copy(i, kb0 + i, unit % m_tiles * ROWS, unit / m_tiles * bn);
     }
     if (warp == 1) {
         if constexpr (PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(tmem_cols) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(p.tmem_cols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(tmem_cols) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(p.tmem_cols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
     tc_fence_before();
     __syncthreads();
+    pdl_wait();                                   // set-up runs beside the end of the kernel before; nothing in memory is read or written until here
     if constexpr (PAIR) cluster_sync_all();       // the peer's barriers exist before anything arrives on them
     tc_fence_after();
     const unsigned tmem_base = tmem_base_s;
 
-    if (warp == 0 && lane == 0) {
-        // ---- producer ---------------------------------------------------------------------------------------
-        int it = 0;
+    if (warp == 0) {
+        // ---- producer: stage s of the ring, in its `turn`-th use (no division: the loops below are chains of a few hundred cycles) --------
+        int it = 0, s = 0;
+        unsigned turn = 0;
         bool gave_up = false;
-        for (long long tile = unit; tile < num_tiles && !gave_up; tile += units) {
-            const int m0 = (int) (tile % m_tiles) * ROWS + (int) rank * TC_BM, n0 = (int) (tile / m_tiles) * bn + (int) rank * half;
+        for (int tile = unit; tile < num_tiles && !gave_up; tile += units) {
+            const int m0 = tile % m_tiles * ROWS + (int) rank * TC_BM, n0 = tile / m_tiles * bn + (int) rank * half;
             for (int kb = kb0; kb < kb1; kb++, it++) {
-                const int s = it % stages;
-                if (!mbar_wait(smem_addr(&empty_bar[s]), ((it / stages) & 1) ^ 1)) { p.status->code = 1; p.status->where = it; gave_up = true; break; }
-                const unsigned to = smem_addr(smem + s * p.stage_bytes);
-                if constexpr (PAIR) {
-                    const unsigned bar = map_to_cta(smem_addr(&full_bar[s]), 0);
-                    if (rank == 0) mbar_expect_tx(smem_addr(&full_bar[s]), 2 * KPS * kb_bytes);
-#pragma unroll
-                    for (int j = 0; j < KPS; j++) {
-                        tma_load_2d_pair(to + j * kb_bytes, &map_a, (kb * KPS + j) * TC_BK, m0, bar);
-                        tma_load_2d_pair(to + j * kb_bytes + a_bytes, &map_b, (kb * KPS + j) * TC_BK, n0, bar);
-                    }
-                } else {
-                    const unsigned bar = smem_addr(&full_bar[s]);
-                    mbar_expect_tx(bar, kb_bytes);
-                    tma_load_2d(to, &map_a, kb * TC_BK, m0, bar);
-                    tma_load_2d(to + a_bytes, &map_b, kb * TC_BK, n0, bar);
+                if (it >= early) {
+                    if (!mbar_wait(smem_addr(&empty_bar[s]), (turn & 1) ^ 1)) { if (lane == 0) { p.status->code = 1; p.status->where = it; } gave_up = true; break; }
+                    copy(s, kb, m0, n0);
                 }
+                if (++s == stages) { s = 0; turn++; }
             }
         }
         if (gave_up) {                            // its copies land before the CTA may leave
             if (rank == 0)
                 for (int i = max(0, it - stages); i < it; i++) mbar_wait(smem_addr(&full_bar[i % stages]), (i / stages) & 1);
         } else if (PAIR) {                        // the last commits still arrive on this CTA's barriers
-            for (int i = 0; i < stages; i++, it++)
-                if (!mbar_wait(smem_addr(&empty_bar[it % stages]), ((it / stages) & 1) ^ 1)) { p.status->code = 5; p.status->where = it; break; }
+            for (int i = 0; i < stages; i++) {
+                if (!mbar_wait(smem_addr(&empty_bar[s]), (turn & 1) ^ 1)) { if (lane == 0) { p.status->code = 5; p.status->where = it; } break; }
+                if (++s == stages) { s = 0; turn++; }
+            }
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
         // ---- MMA issuer -------------------------------------------------------------------------------------
         const unsigned idesc = instr_desc_bf16(ROWS, bn);
-        int it = 0, use = 0;
+        const unsigned long long first = smem_desc_sw128(smem_addr(smem)), to_b = (unsigned long long) (a_bytes >> 4);
+        const unsigned long long next_block = (unsigned long long) (kb_bytes >> 4), next_stage = (unsigned long long) (p.stage_bytes >> 4);
+        unsigned long long at = first;            // (a ring of 208 KB: the descriptor's 14 bits of address do not overflow)
+        int s = 0, use = 0;
+        unsigned turn = 0;
         bool gave_up = false;
-        for (long long tile = unit; tile < num_tiles && !gave_up; tile += units, use++) {
+        for (int tile = unit; tile < num_tiles && !gave_up; tile += units, use++) {
             const int buf = use & 1;
-            if (!mbar_wait(smem_addr(&acc_empty[buf]), ((use >> 1) & 1) ^ 1)) { p.status->code = 4; p.status->where = use; break; }
+            if (!mbar_wait(smem_addr(&acc_empty[buf]), ((use >> 1) & 1) ^ 1)) { if (lane == 0) { p.status->code = 4; p.status->where = use; } break; }
             tc_fence_after();
-            const unsigned d_tmem = tmem_base + (unsigned) (buf * acc_cols);
-            for (int kb = kb0; kb < kb1; kb++, it++) {
-                const int s = it % stages;
-                if (!mbar_wait(smem_addr(&full_bar[s]), (it / stages) & 1)) { p.status->code = 2; p.status->where = it; gave_up = true; break; }
+            const unsigned d_tmem = tmem_base + (unsigned) (buf * p.buf_cols);
+            int a = 0;
+            unsigned more = 0;                    // whether the accumulator already holds sums
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(smem_addr(&full_bar[s]), turn & 1)) { if (lane == 0) { p.status->code = 2; p.status->where = kb; } gave_up = true; break; }
                 tc_fence_after();
 #pragma unroll
                 for (int j = 0; j < KPS; j++) {
-                    const unsigned long long da = smem_desc_sw128(smem_addr(smem + s * p.stage_bytes + j * kb_bytes));
-                    const unsigned long long db = smem_desc_sw128(smem_addr(smem + s * p.stage_bytes + j * kb_bytes + a_bytes));
-#pragma unroll
-                    for (int k = 0; k < TC_BK / 16; k++) {
-                        const unsigned acc = kb > kb0 || j > 0 || k > 0 ? 1u : 0u;
-                        if constexpr (PAIR) tc_mma_pair(d_tmem, da + (unsigned long long) (k * 2), db + (unsigned long long) (k * 2), idesc, acc);
-                        else tc_mma(d_tmem, da + (unsigned long long) (k * 2), db + (unsigned long long) (k * 2), idesc, acc);
-                    }
+                    const unsigned long long da = at + j * next_block, db = da + to_b;
+                    if constexpr (PAIR) tc_mma4_pair(d_tmem + (unsigned) (a * acc_cols), da, db, idesc, more);
+                    else tc_mma4(d_tmem + (unsigned) (a * acc_cols), da, db, idesc, more);
+                    if (++a == p.accs) { a = 0; more = 1; }
                 }
-                if constexpr (PAIR) tc_commit_pair(smem_addr(&empty_bar[s]));
-                else tc_commit(smem_addr(&empty_bar[s]));
+                if constexpr (PAIR) tc_commit_pair_warp(smem_addr(&empty_bar[s]), leader);
+                else tc_commit_warp(smem_addr(&empty_bar[s]));
+                at += next_stage;
+                if (++s == stages) { s = 0; turn++; at = first; }
             }
             if (!gave_up) {
-                if constexpr (PAIR) tc_commit_pair(smem_addr(&acc_full[buf]));
-                else tc_commit(smem_addr(&acc_full[buf]));
+                if constexpr (PAIR) tc_commit_pair_warp(smem_addr(&acc_full[buf]), leader);
+                else tc_commit_warp(smem_addr(&acc_full[buf]));
             }
         }
     } else if (warp >= 2) {
         // ---- epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 -----------------------------------
-        const int q = warp & 3;
+        const int q = warp & 3, half_w = (warp - 2) >> 2;          // the second four warps take every other columns
         const float cap_factor = SCORE && p.score.cap != 0.0f ? 2.0f * kLog2e / p.score.cap : 0.0f;
         int use = 0;
-        for (long long tile = unit; tile < num_tiles; tile += units, use++) {
+        for (int tile = unit; tile < num_tiles; tile += units, use++) {
             const int buf = use & 1;
-            const int n_tile = (int) (tile / m_tiles), m0 = (int) (tile % m_tiles) * ROWS + (int) rank * TC_BM, n0 = n_tile * bn;
+            const int n_tile = tile / m_tiles, m0 = tile % m_tiles * ROWS + (int) rank * TC_BM, n0 = n_tile * bn;
+            const int row = m0 + q * 32 + lane, cols = min(bn, p.N - n0);
+            if constexpr (!SCORE) {
+                if (p.epi.res != nullptr && row < p.T) {          // the residual's lines come into the L2 while the products run
+                    const int size = p.epi.res_bf16 ? 2 : 4;
+                    const char * line = (const char *) p.epi.res + ((size_t) row * p.epi.ldr + n0) * size;
+                    for (int b = half_w * 128; b < cols * size; b += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + b));
+                }
+            }
             if (!mbar_wait(smem_addr(&acc_full[buf]), (use >> 1) & 1)) {
                 if (lane == 0) { p.status->code = 3; p.status->where = use; }
                 break;
             }
             tc_fence_after();
-            const int row = m0 + q * 32 + lane, cols = min(bn, p.N - n0);
-            const unsigned acc = tmem_base + ((unsigned) (q * 32) << 16) + (unsigned) (buf * acc_cols);
+            const unsigned acc = tmem_base + ((unsigned) (q * 32) << 16) + (unsigned) (buf * p.buf_cols);
             if (m0 + q * 32 < p.T) {              // (a warp whose rows are all behind the last one has nothing to do)
                 if constexpr (SCORE) {
                     float m = -CUDART_INF_F, s = 0.0f;
                     const int wanted = row < p.T ? p.score.targets[row] : -1, target = wanted < 0 ? -1 : wanted - n0;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < cols; c0 += 32) {
+                    for (int c0 = half_w * 32; c0 < cols; c0 += 64) {
                         unsigned r[32];
                         tc_ld32(acc + (unsigned) c0, r);
                         tc_wait_ld();
+                        if (p.accs == 2) {
+                            unsigned r2[32];
+                            tc_ld32(acc + (unsigned) (acc_cols + c0), r2);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
+                        }
                         lf_take(r, cols - c0, p.score.cap, cap_factor, m, s);
                         if (target >= c0 && target < c0 + 32 && target < cols) {
                             const float z = __uint_as_float(lf_pick(r, target - c0));
                             p.score.lp[row] = p.score.cap != 0.0f ? p.score.cap * tanhf(z / p.score.cap) : z;
                         }
                     }
-                    if (row < p.T) p.score.part[(size_t) n_tile * p.T + row] = make_float2(m, s);
-                } else if (PAIR || p.ks == 1) {
-#pragma unroll 1
-                    for (int c0 = 0; c0 < cols; c0 += 32) {
-                        unsigned r[32];
-                        tc_ld32(acc + (unsigned) c0, r);
-                        tc_wait_ld();
-                        if (row < p.T) {
+                    if (row < p.T) p.score.part[((size_t) n_tile * 2 + half_w) * p.T + row] = make_float2(m, s);
+                } else if (p.ks == 1) {
+                    // 32 rows of LF_COLS columns at a time, turned around in shared memory: a lane then holds 4 columns of every LF_TURN-th row, so
+                    // that the residual is read and the result written whole lines at a time.  The residual is asked for before the sums.
+                    float * turn = reinterpret_cast<float *>(smem + kLfRing) + (warp - 2) * 32 * LF_COLS;
+                    const int in_row = lane / (LF_COLS / 4), in_col = lane % (LF_COLS / 4) * 4, row0 = m0 + q * 32;
+                    auto residual = [&](int c0, float4 (&res)[LF_TURNS]) {
 #pragma unroll
-                            for (int v = 0; v < 4; v++) {
-                                const int live = cols - c0 - 8 * v;
-                                if (live > 0) {
-                                    float y[8];
-#pragma unroll
-                                    for (int i = 0; i < 8; i++) y[i] = __uint_as_float(r[8 * v + i]);
-                                    p.epi.store8(y, row, n0 + c0 + 8 * v, live);
-                                }
-                            }
+                        for (int i = 0; i < LF_TURNS; i++) {
+                            const int r0 = row0 + in_row + i * LF_TURN;
+                            res[i] = lf_residual<KIND>(p.epi, (size_t) r0, n0 + c0 + in_col, r0 < p.T ? cols - c0 - in_col : 0);
                         }
-                    }
-                } else {
-                    // this CTA's part of the sums, for the cluster: rows of bn + 4 floats over the ring, whose copies and products are all done
-                    float * part = reinterpret_cast<float *>(smem) + (size_t) (q * 32 + lane) * (bn + 4);
+                    };
+                    float4 res[LF_TURNS], next[LF_TURNS];
+                    residual(half_w * LF_COLS, next);
 #pragma unroll 1
-                    for (int c0 = 0; c0 < bn; c0 += 32) {
-                        unsigned r[32];
-                        tc_ld32(acc + (unsigned) c0, r);
-                        tc_wait_ld();
-                        if (row < p.T) {
+                    for (int c0 = half_w * LF_COLS; c0 < cols; c0 += LF_WARPS / 4 * LF_COLS) {
+                        const int live = cols - c0 - in_col, col = n0 + c0 + in_col;
 #pragma unroll
-                            for (int v = 0; v < 8; v++)
-                                if (c0 + 4 * v < bn) *reinterpret_cast<uint4 *>(part + c0 + 4 * v) = make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+                        for (int i = 0; i < LF_TURNS; i++) res[i] = next[i];
+                        residual(c0 + LF_WARPS / 4 * LF_COLS, next);
+                        const float4 bias = lf_bias<KIND>(p.epi, col, live);
+                        float r[LF_COLS];
+                        lf_sum(acc + (unsigned) c0, p.accs, acc_cols, r);
+                        __syncwarp();                                   // the columns before have been read
+#pragma unroll
+                        for (int v = 0; v < LF_COLS / 4; v++)
+                            *reinterpret_cast<float4 *>(turn + lane * LF_COLS + (v ^ ((lane >> 1) & 3)) * 4) = make_float4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+                        __syncwarp();
+                        float y[4 * LF_TURNS];
+#pragma unroll
+                        for (int i = 0; i < LF_TURNS; i++) {
+                            const float4 v = *reinterpret_cast<const float4 *>(turn + (in_row + i * LF_TURN) * LF_COLS + (in_col ^ (((in_row + i * LF_TURN) >> 1) & 3) * 4));
+                            y[4 * i] = v.x + bias.x; y[4 * i + 1] = v.y + bias.y; y[4 * i + 2] = v.z + bias.z; y[4 * i + 3] = v.w + bias.w;
+                        }
+                        linear_act_values<4 * LF_TURNS>(y, p.epi.act);
+#pragma unroll
+                        for (int i = 0; i < LF_TURNS; i++) {
+                            const int r0 = row0 + in_row + i * LF_TURN;
+                            lf_put<KIND>(p.epi, y + 4 * i, res[i], (size_t) r0, col, r0 < p.T ? live : 0);
                         }
                     }
                 }
@@ -263,7 +367,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) linear_fused_kernel(const __gri
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(smem_addr(&acc_empty[buf]), 0));
+                if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(smem_addr(&acc_empty[buf]), leader));
                 else mbar_arrive(smem_addr(&acc_empty[buf]));
             }
         }
@@ -272,39 +376,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1) linear_fused_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     __syncwarp();
-    if constexpr (!PAIR && !SCORE) {
+    if constexpr (!SCORE) {
         if (p.ks > 1) {
-            cluster_sync_all();                   // all parts lie ready
-            const int m0 = (unit % m_tiles) * ROWS, n0 = (unit / m_tiles) * bn;
-            const int rows = min(TC_BM, p.T - m0), cols = min(bn, p.N - n0), per_row = (cols + 7) / 8;
-            const int pieces = rows * per_row, from = (int) ((long long) pieces * cluster_rank / p.ks), to = (int) ((long long) pieces * (cluster_rank + 1) / p.ks);
-            const unsigned base = smem_addr(smem);
-            for (int i = from + (int) threadIdx.x; i < to; i += TC_THREADS) {
-                const int row = i / per_row, c = (i - row * per_row) * 8;
-                const unsigned at = base + (unsigned) (row * (bn + 4) + c) * 4u;
-                float y[8];
+            if (p.recv_shared) cluster_sync_all();            // every CTA's ring is done with
+            const int m0 = unit % m_tiles * ROWS + (int) rank * TC_BM, n0 = unit / m_tiles * bn, rows = min(TC_BM, p.T - m0);
+            const unsigned recv = smem_addr(smem) + (unsigned) p.recv_off;
+            if (warp >= 2) {
+                // this CTA's sums go to the CTAs that add them up, 4 columns a store; stores to another SM need no answer, where loads from there
+                // waited a microsecond each time round (128 x 4,096 x 4,096 18.5 us)
+                tc_fence_after();
+                const int q = warp & 3, row = q * 32 + lane;
+                const unsigned acc = tmem_base + ((unsigned) (q * 32) << 16), mine = recv + (unsigned) ((split * p.recv_rows + row) * p.recv_ld) * 16u;
+                if (q * 32 < rows) {
+#pragma unroll 1
+                    for (int c0 = (warp - 2) / 4 * LF_COLS; c0 < bn; c0 += LF_WARPS / 4 * LF_COLS) {
+                        float r[LF_COLS];
+                        lf_sum(acc + (unsigned) c0, p.accs, acc_cols, r);
+                        if (row < rows) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = 0.0f;
-#pragma unroll 4
-                for (int r = 0; r < p.ks; r++) {
-                    const unsigned peer = map_to_cta(at, (unsigned) r);
-                    float a[8];
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]) : "r"(peer) : "memory");
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]) : "r"(peer + 16) : "memory");
-#pragma unroll
-                    for (int j = 0; j < 8; j++) y[j] += a[j];
+                            for (int v = 0; v < LF_COLS / 4; v++) {
+                                const int i = c0 / 4 + v, owner = (i * p.inv_per) >> 16;
+                                const unsigned to = map_to_cta(mine + (unsigned) (i - owner * p.per) * 16u, PAIR ? 2u * owner + rank : (unsigned) owner);
+                                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(r[4 * v]), "f"(r[4 * v + 1]), "f"(r[4 * v + 2]), "f"(r[4 * v + 3]) : "memory");
+                            }
+                        }
+                    }
                 }
-                p.epi.store8(y, (size_t) (m0 + row), n0 + c, cols - c);
+                tc_fence_before();
+                __syncwarp();
             }
-            __syncwarp();
-            cluster_sync_all();                   // nobody leaves while its part is read
+            cluster_sync_all();                               // all parts have arrived; nobody reaches into another's memory from here on
+            const int from = split * p.per, width = min(p.per, (min(bn, p.N - n0) + 3) / 4 - from), pieces = width > 0 ? max(rows, 0) * width : 0;
+            const float4 * part = reinterpret_cast<const float4 *>(smem + p.recv_off);
+            for (int i = threadIdx.x; i < pieces; i += LF_THREADS) {
+                const int row = i / width, c = i - row * width, col = n0 + (from + c) * 4, live = p.N - col;
+                const float4 bias = lf_bias<KIND>(p.epi, col, live), res = lf_residual<KIND>(p.epi, (size_t) (m0 + row), col, live);
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = 0; r < p.ks; r++) {
+                    const float4 v = part[(r * p.recv_rows + row) * p.recv_ld + c];
+                    y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
+                }
+                y[0] += bias.x; y[1] += bias.y; y[2] += bias.z; y[3] += bias.w;
+                linear_act_values<4>(y, p.epi.act);
+                lf_put<KIND>(p.epi, y, res, (size_t) (m0 + row), col, live);
+            }
         }
     }
-    if constexpr (PAIR) cluster_sync_all();
+    if constexpr (PAIR) {
+        if (p.ks == 1) cluster_sync_all();        // neither frees tensor memory or leaves while the other may use its memory
+    }
     if (warp == 1) {
         tc_fence_after();
-        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.tmem_cols) : "memory");
     }
 }
 
@@ -313,6 +437,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) linear_fused_kernel(const __gri
 __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __restrict__ part, int n_tiles, int T, int V, int rows,
                                                             const int * __restrict__ targets, float * __restrict__ lp, float * __restrict__ lse) {
     __shared__ float sm[512], ss[512];
+    pdl_launch_dependents();
+    pdl_wait();
     const int r = threadIdx.x & (rows - 1), seg = threadIdx.x / rows, segs = 512 / rows;
     const long long row = (long long) blockIdx.x * rows + r;
     float m = -CUDART_INF_F, s = 0.0f;
@@ -351,6 +477,8 @@ __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __res
 __global__ void __launch_bounds__(256) logprobs_piece_kernel(const float * __restrict__ logits, int T, int P, int v0, const int * __restrict__ targets,
                                                              float * __restrict__ lp, float2 * __restrict__ part, int first, float cap) {
     __shared__ float sm[8], ss[8];
+    pdl_launch_dependents();
+    pdl_wait();
     const size_t row = blockIdx.x;
     const int splits = gridDim.y, c0 = (int) ((long long) P * blockIdx.y / splits), c1 = (int) ((long long) P * (blockIdx.y + 1) / splits);
     const float * z = logits + row * P;
@@ -386,8 +514,7 @@ __global__ void __launch_bounds__(256) logprobs_piece_kernel(const float * __res
 static int lf_join(const float * part, int n_tiles, int T, int V, const int * targets, float * lp, float * lse, cudaStream_t stream) {
     int rows = 1;
     while (rows < 32 && rows < T) rows *= 2;
-    logprobs_join_kernel<<<(unsigned) ((T + rows - 1) / rows), 512, 0, stream>>>((const float2 *) part, n_tiles, T, V, rows, targets, lp, lse);
-    return iian_launch_status();
+    return iian_launch(logprobs_join_kernel, dim3((unsigned) ((T + rows - 1) / rows)), dim3(512), 0, stream, (const float2 *) part, n_tiles, T, V, rows, targets, lp, lse);
 }
 
 // SMs of the current device, asked for once
@@ -401,43 +528,77 @@ static int lf_sms() {
     return n;
 }
 
-// bn, ks as given; pair: tiles of 256 rows on pairs of SMs.
-template <bool PAIR, bool SCORE>
-static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, int sms, cudaStream_t stream) {
+// T, N, bn, ks, status, epi or score as given; PAIR: tiles of 256 rows on pairs of SMs.
+template <bool PAIR, int KIND>
+static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, int K, int sms, cudaStream_t stream) {
     constexpr int KPS = PAIR ? 2 : 1, ROWS = PAIR ? 2 * TC_BM : TC_BM;
     // All of it whatever the call needs: two CTAs of a cluster that each waited for the tensor memory of an SM's other CTA, those two in turn
     // waiting for their clusters, would never end, so no SM may hold two.
-    constexpr int kRing = 208 * 1024, smem = kRing + 1024;
-    p.a_rows = PAIR || p.T >= TC_BM ? TC_BM : (p.T + 7) / 8 * 8;
-    const int half = PAIR ? p.bn / 2 : p.bn;
-    p.stage_bytes = KPS * (p.a_rows + half) * TC_BK * 2;
-    const int over = (TC_BM - p.a_rows) * TC_BK * 2;                   // the last stage's product reads 128 rows too
-    p.stages = std::min(LF_STAGES, (kRing - over) / p.stage_bytes);
-    static_assert(TC_BM * (256 + 4) * 4 <= kRing, "a tile's sums fit the ring");
-    auto kernel = linear_fused_kernel<PAIR, SCORE>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr int kRing = kLfRing, smem = kLfSmem, kRecvMost = 80 * 1024;
+    const int a_rows = PAIR || p.T >= TC_BM ? TC_BM : (p.T + 7) / 8 * 8, half = PAIR ? p.bn / 2 : p.bn;
+    p.a_bytes = a_rows * TC_BK * 2;
+    p.kb_bytes = p.a_bytes + half * TC_BK * 2;
+    p.stage_bytes = KPS * p.kb_bytes;
+    const int over = (TC_BM - a_rows) * TC_BK * 2;                     // the last stage's product reads 128 rows too
+    int ring = kRing;
+    if (p.ks > 1) {
+        p.per = (p.bn / 4 + p.ks - 1) / p.ks;
+        p.inv_per = (65536 + p.per - 1) / p.per;
+        p.recv_ld = p.per | 1;                                         // an odd number of 16-byte groups: rows of eight lanes meet no bank twice
+        p.recv_rows = a_rows;
+        const int recv = p.ks * a_rows * p.recv_ld * 16;
+        if (recv > kRing) return IIAN_ERR_SHAPE;
+        p.recv_shared = recv > kRecvMost;
+        if (!p.recv_shared) ring = (kRing - recv) / 1024 * 1024;
+        p.recv_off = p.recv_shared ? 0 : ring;
+    }
+    p.stages = std::min(LF_STAGES, (ring - over) / p.stage_bytes);
+    p.all_kb = ((K + TC_BK - 1) / TC_BK + KPS - 1) / KPS;
+    p.m_tiles = (p.T + ROWS - 1) / ROWS;
+    const long long tiles = (long long) p.m_tiles * ((p.N + p.bn - 1) / p.bn);
+    const int group = (PAIR ? 2 : 1) * p.ks;
+    if (tiles * group > 2147483647LL - 65536) return IIAN_ERR_LIMIT;
+    p.num_tiles = (int) tiles;
+    p.units = p.ks > 1 ? p.num_tiles : std::min(p.num_tiles, sms / group);
+    const int acc_cols = (p.bn + 31) & ~31, bufs = p.units < p.num_tiles ? 2 : 1;      // (a CTA with one tile needs no second buffer)
+    p.accs = 1;
+    while (p.accs < (KIND == LF_SCORE ? 2 : 4) && 2 * p.accs * bufs * acc_cols <= 512 && 2 * p.accs <= p.all_kb / p.ks) p.accs *= 2;
+    p.buf_cols = p.accs * acc_cols;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < (unsigned) (bufs * p.buf_cols)) p.tmem_cols *= 2;
+    auto kernel = linear_fused_kernel<PAIR, KIND>;
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !configured[dev])) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+    }
     if (e != cudaSuccess) return 1000 + (int) e;
     CUtensorMap ma, mb;
-    int rc = make_map(&ma, x, p.T, p.K, p.a_rows, ldx);
+    int rc = make_map(&ma, x, p.T, K, a_rows, ldx);
     if (rc != IIAN_OK) return rc;
-    rc = make_map(&mb, w, p.N, p.K, half);
+    rc = make_map(&mb, w, p.N, K, half);
     if (rc != IIAN_OK) return rc;
-    const long long tiles = (long long) ((p.T + ROWS - 1) / ROWS) * ((p.N + p.bn - 1) / p.bn);
-    const int group = PAIR ? 2 : p.ks;
-    const long long units = p.ks > 1 ? tiles : std::min<long long>(tiles, sms / group);
-    if (units * group > 2147483647LL) return IIAN_ERR_LIMIT;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (units * group));
-    cfg.blockDim = dim3(TC_THREADS);
+    cfg.gridDim = dim3((unsigned) (p.units * group));
+    cfg.blockDim = dim3(LF_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned) group;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    unsigned attrs = 0;
+    if (group > 1) {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = (unsigned) group;
+        attr[attrs].val.clusterDim.y = 1;
+        attr[attrs++].val.clusterDim.z = 1;
+    }
+    if (g_iian_pdl) {
+        attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = group > 1 ? 1 : 0;
+    cfg.numAttrs = attrs;
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, (const LfArgs) p);
     return e == cudaSuccess ? IIAN_OK : 1000 + (int) e;
 }
@@ -451,12 +612,54 @@ static int lf_check(int T, int N, int K, const void * x, long long ldx, const vo
 
 static int lf_even(int n, int parts, int step) { return std::max(32, ((n + parts - 1) / parts + step - 1) / step * step); }
 
+// The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants are fitted to 26 shapes from
+// 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024, each timed in every form (the form it takes is 2 % slower than the best one on average, 11 % at
+// most).  A K block costs the longest of its copies (128 GB/s an SM, 17 TB/s together), its products, and 0.26 us that a block's
+// instructions and commit take; the operands come from memory at 4.9 TB/s; then come the epilogue of a tile and, where K is shared, the exchange of
+// the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
+static double lf_estimate(int T, int N, int K, int sms, bool pair, int bn, int ks) {
+    const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8;
+    const double tiles = (double) ((T + rows - 1) / rows) * ((N + bn - 1) / bn), ctas = tiles * ks * group;
+    int slots = sms / (group * ks) * (group * ks);
+    if (ks > 4) slots = std::min(slots, sms - sms / 9);          // clusters of six or eight leave some SMs of a GPC over
+    const double waves = (double) (long long) ((ctas + slots - 1) / slots), active = std::min(ctas, (double) slots);
+    const int kb = ((K + TC_BK - 1) / TC_BK + ks - 1) / ks;
+    const double fill = (a_rows + (pair ? bn / 2 : bn)) * 128.0 / std::min(128e3, 17.1e6 / active), mma = std::max(0.263, bn * 2 / 1850.0 * 1.54);
+    double t = std::max(waves * kb * std::max(fill, mma), 2.0 * K * ((double) N + T) / 4.89e6);
+    if (ks == 1) t += 3.15 * bn / 256 * (a_rows / 128.0 * 0.225 + 0.775);
+    else t += 1.44 + waves * 11.1 * ks * a_rows * (((bn / 4 + ks - 1) / ks) | 1) * 16 / 131072.0;
+    return t;
+}
+static void lf_plan(int T, int N, int K, int sms, bool out_f32, bool * pair, int * bn, int * ks) {
+    struct Known { int T, N, K, sms, f32, pair, bn, ks; };
+    static thread_local Known known[16] = {};                // by sizes alone: a model's few products come again and again
+    Known & k = known[((unsigned) T * 31u + (unsigned) N * 7u + (unsigned) K) % 16u];
+    if (!(k.T == T && k.N == N && k.K == K && k.sms == sms && k.f32 == (int) out_f32 && k.bn > 0)) {
+        static const int columns[] = {32, 48, 64, 96, 112, 128, 160, 192, 224, 256}, shares[] = {1, 2, 3, 4, 6};
+        const int blocks = (K + TC_BK - 1) / TC_BK, most = out_f32 && K > 6144 ? 128 : 256;
+        double best = 1e300;
+        for (int p = 0; p < (T > TC_BM ? 2 : 1); p++)
+            for (int c : columns)
+                for (int s : shares) {
+                    if (c > most || (p && c % 32 != 0) || s > (p ? 4 : 6) || s > (p ? (blocks + 1) / 2 : blocks)) continue;
+                    const long long ctas = (long long) ((T + (p ? 255 : 127)) / (p ? 256 : 128)) * ((N + c - 1) / c) * (p ? 2 : 1);
+                    if (s > 1 && ctas >= sms) break;
+                    const double t = lf_estimate(T, N, K, sms, p != 0, c, s);
+                    if (t < best) { best = t; k = {T, N, K, sms, (int) out_f32, p, c, s}; }
+                    if (c > N) break;
+                }
+    }
+    *pair = k.pair != 0;
+    *bn = k.bn;
+    *ks = k.ks;
+}
+
 }  // namespace iian
 
 using namespace iian;
 
 // x [T, K] bf16, rows ldx apart; w [N, K] bf16; status: two ints the host reads, as for iian_gemm_tcgen05.  form 0: chosen here; else
-// pair | bn << 1 | ks << 16 (a multiple of 16 from 32 to 256, on pairs of 32; 1 to 8 CTAs that share K, 1 on pairs).
+// pair | bn << 1 | ks << 16 (a multiple of 16 from 32 to 256, on pairs of 32; 1 to 8 CTAs that share K, or 1 to 4 pairs).
 IIAN_API int iian_linear_act(const void * x, long long ldx, const void * w, const float * bias, const void * residual, int res_dtype,
                              long long ldr, void * out, int out_dtype, long long ldo, int T, int N, int K, int act, int form, int * status,
                              cudaStream_t stream) {
@@ -466,26 +669,29 @@ IIAN_API int iian_linear_act(const void * x, long long ldx, const void * w, cons
     LfArgs p = {};
     if (!linear_epilogue(p.epi, bias, residual, res_dtype, ldr, out, out_dtype, ldo, act)) return IIAN_ERR_DTYPE;
     const int sms = lf_sms();
-    p.T = T; p.N = N; p.K = K;
+    p.T = T; p.N = N;
     p.status = (TcStatus *) status;
     const int blocks = (K + TC_BK - 1) / TC_BK;
-    bool pair = T > TC_BM;
-    p.bn = pair ? 256 : lf_even(N, (N + 127) / 128, 16);
-    p.ks = 1;
-    if (!pair) {
-        const int tiles = (N + p.bn - 1) / p.bn;
-        while (p.ks < 8 && tiles * p.ks * 2 <= sms && blocks >= p.ks * 4) p.ks *= 2;
-    }
+    bool pair = false;
+    if (form == 0) lf_plan(T, N, K, sms, out_dtype == IIAN_F32, &pair, &p.bn, &p.ks);
     if (form != 0) {
         pair = form & 1;
         p.bn = (form >> 1) & 0x7fff;
         p.ks = form >> 16;
-        if (p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0 || p.ks < 1 || p.ks > (pair ? 1 : 8) || p.ks > blocks) return IIAN_ERR_SHAPE;
+        if (p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0 || p.ks < 1 || p.ks > (pair ? 4 : 8) || p.ks > (pair ? (blocks + 1) / 2 : blocks) || (p.ks > 1 && p.bn / 4 < p.ks)) return IIAN_ERR_SHAPE;
     }
-    return pair ? lf_launch<true, false>(p, x, ldx, w, sms, stream) : lf_launch<false, false>(p, x, ldx, w, sms, stream);
+    const LinearEpilogue & e = p.epi;
+    const bool whole = N % 4 == 0 && e.out_vec && (bias == nullptr || e.bias_vec) && (residual == nullptr || (e.res_vec && !e.res_bf16));
+    auto go = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
+        return pair ? lf_launch<true, KIND>(p, x, ldx, w, K, sms, stream) : lf_launch<false, KIND>(p, x, ldx, w, K, sms, stream);
+    };
+    if (!whole) return go(std::integral_constant<int, LF_ANY>());
+    if (residual == nullptr) return e.out_bf16 ? go(std::integral_constant<int, LF_BF16>()) : go(std::integral_constant<int, LF_F32>());
+    return e.out_bf16 ? go(std::integral_constant<int, LF_BF16_RES>()) : go(std::integral_constant<int, LF_F32_RES>());
 }
 
-// Column tiles of a call, whose partial sums take 8 bytes a tile and row; form as above (0: the one chosen), ks 1.
+// Partial sums of a row (8 bytes each) that a call leaves; form as above (0: the one chosen), ks 1.
 static int lf_score_form(int T, int N, int form, bool * pair) {
     const int sms = lf_sms();
     *pair = T > TC_BM;
@@ -502,7 +708,7 @@ IIAN_API int iian_linear_logprobs_tiles(int T, int N, int form) {
     if (T <= 0 || N <= 0) return 0;
     bool pair;
     const int bn = lf_score_form(T, N, form, &pair);
-    return bn < 32 ? 0 : (N + bn - 1) / bn;
+    return bn < 32 ? 0 : 2 * ((N + bn - 1) / bn);
 }
 
 // targets [T]; lp, lse [T] float32; part: [tiles][T] pairs of floats, tiles as iian_linear_logprobs_tiles says.
@@ -516,15 +722,15 @@ IIAN_API int iian_linear_logprobs(const void * x, long long ldx, const void * w,
     LfArgs p = {};
     const int sms = lf_sms();
     bool pair;
-    p.T = T; p.N = N; p.K = K;
+    p.T = T; p.N = N;
     p.bn = lf_score_form(T, N, form, &pair);
     p.ks = 1;
     if (p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0) return IIAN_ERR_SHAPE;
     p.status = (TcStatus *) status;
     p.score = {(float2 *) part, targets, lp, cap};
-    rc = pair ? lf_launch<true, true>(p, x, ldx, w, sms, stream) : lf_launch<false, true>(p, x, ldx, w, sms, stream);
+    rc = pair ? lf_launch<true, LF_SCORE>(p, x, ldx, w, K, sms, stream) : lf_launch<false, LF_SCORE>(p, x, ldx, w, K, sms, stream);
     if (rc != IIAN_OK) return rc;
-    return lf_join(part, (N + p.bn - 1) / p.bn, T, N, targets, lp, lse, stream);
+    return lf_join(part, 2 * ((N + p.bn - 1) / p.bn), T, N, targets, lp, lse, stream);
 }
 
 // The same from logits in memory, a piece of the vocabulary at a time: logits [T, P] float32 hold columns v0 .. v0 + P, whose `splits` parts
@@ -533,8 +739,7 @@ IIAN_API int iian_linear_logprobs_piece(const float * logits, int T, int P, int 
                                         int splits, float cap, cudaStream_t stream) {
     if (T <= 0 || P <= 0) return IIAN_OK;
     if (splits <= 0 || splits > 65535 || first < 0 || cap < 0.0f) return IIAN_ERR_SHAPE;
-    logprobs_piece_kernel<<<dim3((unsigned) T, (unsigned) splits), 256, 0, stream>>>(logits, T, P, v0, targets, lp, (float2 *) part, first, cap);
-    return iian_launch_status();
+    return iian_launch(logprobs_piece_kernel, dim3((unsigned) T, (unsigned) splits), dim3(256), 0, stream, logits, T, P, v0, targets, lp, (float2 *) part, first, cap);
 }
 IIAN_API int iian_linear_logprobs_join(const float * part, int parts, int T, int V, const int * targets, float * lp, float * lse, cudaStream_t stream) {
     if (T <= 0) return IIAN_OK;

@@ -30,6 +30,8 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __
                                                                 const float * __restrict__ correction, int E, int groups, int lanes,
                                                                 int top_groups, int group_top, int top, int softmax, int renorm,
                                                                 double scale, int * __restrict__ ids, float * __restrict__ wts, int N) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const long long t = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (t >= N) return;
@@ -154,9 +156,8 @@ IIAN_API int iian_moe_route_grouped(const float * logits, long long ld, const fl
     const int lanes = 32 / wide, slots = (E / groups + lanes - 1) / lanes, warps = 4;
     const dim3 grid((unsigned) (((long long) N + warps - 1) / warps));
     auto go = [&](auto kernel) {
-        kernel<<<grid, warps * 32, 0, stream>>>(logits, ld, correction, E, groups, lanes, top_groups, group_top, top, softmax, renorm,
-                                                (double) scale, ids, wts, N);
-        return iian_launch_status();
+        return iian_launch(kernel, grid, dim3(warps * 32), 0, stream, logits, ld, correction, E, groups, lanes, top_groups, group_top, top,
+                           softmax, renorm, (double) scale, ids, wts, N);
     };
     if (slots <= 2) return go(moe_route_grouped_kernel<2>);
     if (slots <= 4) return go(moe_route_grouped_kernel<4>);

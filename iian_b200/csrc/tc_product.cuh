@@ -113,6 +113,48 @@ __device__ __forceinline__ void tc_mma_pair(unsigned d_tmem, unsigned long long 
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// ---- the same issued by a whole warp, of which one lane is elected ------------------------------------------------
+// Inside a branch that one lane takes, the compiler has to bring every operand of a matrix instruction or copy into a uniform register by
+// itself (600 cycles for the four instructions and the commit of a K block); a warp that runs the loop as one keeps them there.
+__device__ __forceinline__ void tc_mma4(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 a, b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+                 " add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+                 " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+                 " add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_mma4_pair(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p, q, t;\n .reg .b64 a, b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+                 " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+                 " add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n @q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n"
+                 " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n @q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n"
+                 " add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n @q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_commit_warp(unsigned bar) {
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+                 ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_commit_pair_warp(unsigned bar, unsigned leader) {      // to the pair of CTAs leader, leader + 1 of the cluster
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+                 " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}"
+                 ::"r"(bar), "h"((unsigned short) (3u << leader)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_warp(unsigned bar, unsigned bytes) {
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_warp(unsigned dst, const CUtensorMap * map, int x, int y, unsigned bar) {
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+                 " @q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair_warp(unsigned dst, const CUtensorMap * map, int x, int y, unsigned bar_cluster) {
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+                 " @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar_cluster) : "memory");
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

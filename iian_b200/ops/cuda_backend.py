@@ -111,7 +111,7 @@ _sigs_done = set()
 # takes nearly all of an SM's shared memory, so it only becomes resident where one has left): 3.10 -> 2.91 ms per decode
 # step at batch 1, 3.60 -> 3.31 at batch 8.  With the attribute on every kernel of the step the register-bound kernels
 # of the chain did lose resources to their successors (4.16 ms at batch 1 when the products were of that kind).
-_PDL_ENV = os.environ.get("IIAN_PDL", "gemm_stream")
+_PDL_ENV = os.environ.get("IIAN_PDL", "gemm_stream,linear_fused,moe_groups")
 PDL = _PDL_ENV not in ("0", "false", "off")
 _PDL_LIBS = None if _PDL_ENV in ("0", "false", "off", "1", "true", "on") else {n.strip() for n in _PDL_ENV.split(",")}
 
