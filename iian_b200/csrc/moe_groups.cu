@@ -5,9 +5,13 @@
 //   of the `top_groups` groups with the largest scores (ties: the lower group) the `top` outputs with the largest c (ties: the lower index)
 //   w = s, without the correction; with `renorm` divided by the sum of the chosen s; times `scale`
 //
-// Scores are formed and compared in 64 bits: which of two neighbouring scores is the larger is a whole number, and the rounding of a
-// 32-bit exponential would decide it.  A score that is no number is the smallest; a row whose chosen scores are all 0 weighs 0
-// (a softmax over logits of minus infinity alone is such a row).
+// Which of two scores is the larger is a whole number, and the rounding of a 32-bit exponential would decide it where they are neighbours.  So
+// the order is that of the scores in 64 bits: a warp forms them in 32, and where two scores whose order matters are nearer to one another
+// than these can tell, does its token again in 64.  A score that is no number is the smallest; a row whose chosen scores are all 0
+// weighs 0 (a softmax over logits of minus infinity alone is such a row).
+//
+// What bounds it: the integer pipe, that is the chain of `top` reductions and the groups' ranks.  8,192 tokens, 8 of 256 experts in 8 groups: 14.5 us, 24
+// with all scores in 64 bits; a decode step's 61 tokens 2.8, the launch.
 #include "common.cuh"
 
 namespace iian {
@@ -22,32 +26,44 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
     return (unsigned long long) (b ^ ((b >> 63) | (long long) 0x8000000000000000ull));
 }
 
-// One warp a token.  Every group has `lanes` = 32 / (groups, rounded up to a power of two) lanes of its own, output g * per + sub + lanes * i
-// lies in slot i of lane g * lanes + sub: a group's best two are a reduction over its own lanes, and a group's rank among the groups is
-// a count.  The choice is a chain of `top` reductions over the warp; lane k keeps choice k.
+__device__ __forceinline__ unsigned order_key(float v) {
+    const int b = __float_as_int(v);
+    return (unsigned) (b ^ ((b >> 31) | (int) 0x80000000u));
+}
+
+__device__ __forceinline__ float route_sigmoid(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + __expf(-x)));
+    return y;
+}
+
+struct RouteArgs {
+    const float * logits;
+    long long ld;
+    const float * correction;
+    int E, groups, lanes, chunk, top_groups, group_top, top, softmax, renorm;
+    double scale;
+    int * ids;
+    float * wts;
+};
+
+// One warp a token.  Every group has `lanes` = 32 / (groups, rounded up to a power of two) lanes of its own, each with `chunk` neighbouring
+// outputs: a group's best two are a reduction over its own lanes, and a group's rank among the groups is a count.  The choice is a
+// chain of `top` reductions over the warp; lane k keeps choice k.
 template <int SLOTS>
-__global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __restrict__ logits, long long ld,
-                                                                const float * __restrict__ correction, int E, int groups, int lanes,
-                                                                int top_groups, int group_top, int top, int softmax, int renorm,
-                                                                double scale, int * __restrict__ ids, float * __restrict__ wts, int N) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long t = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (t >= N) return;
-    const int per = E / groups, group = lane / lanes, sub = lane - group * lanes, first = group * per;
-    const bool live = group < groups;
-    const float * z = logits + t * ld;
+__device__ __noinline__ void route_exact(const RouteArgs & p, long long t) {
+    const int lane = threadIdx.x & 31, per = p.E / p.groups, group = lane / p.lanes, j0 = (lane - group * p.lanes) * p.chunk;
+    const int first = group * per + j0, held = group < p.groups ? max(0, min(p.chunk, per - j0)) : 0;
+    const float * z = p.logits + t * p.ld + first;
     double s[SLOTS];
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < SLOTS; i++) {
-        const int j = sub + lanes * i;
-        const float v = live && j < per ? z[first + j] : -INFINITY;
+        const float v = i < held ? z[i] : -INFINITY;
         s[i] = v;
         mx = fmaxf(mx, v);
     }
-    if (softmax) {
+    if (p.softmax) {
         mx = warp_max(mx);
         if (mx == -INFINITY) mx = 0.0f;                      // nothing but minus infinity: every score 0
         double sum = 0.0;
@@ -69,10 +85,9 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __
     double b1 = -INFINITY, b2 = -INFINITY;                   // this lane's two largest c
 #pragma unroll
     for (int i = 0; i < SLOTS; i++) {
-        const int j = sub + lanes * i;
         key[i] = 0;
-        if (live && j < per) {
-            double c = correction != nullptr ? s[i] + (double) correction[first + j] : s[i];
+        if (i < held) {
+            double c = p.correction != nullptr ? s[i] + (double) p.correction[first + i] : s[i];
             if (c != c) c = -INFINITY;
             c += 0.0;                                        // minus zero is zero
             key[i] = order_key(c);
@@ -80,20 +95,20 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __
             b1 = fmax(b1, c);
         }
     }
-    if (top_groups < groups) {
-        for (int o = 1; o < lanes; o <<= 1) {
+    if (p.top_groups < p.groups) {
+        for (int o = 1; o < p.lanes; o <<= 1) {
             const double o1 = shfl_xor_f64(b1, o), o2 = shfl_xor_f64(b2, o);
             b2 = fmax(fmax(b2, o2), fmin(b1, o1));
             b1 = fmax(b1, o1);
         }
-        double gs = group_top == 2 && per > 1 ? b1 + b2 : b1;
+        double gs = p.group_top == 2 && per > 1 ? b1 + b2 : b1;
         if (gs != gs) gs = -INFINITY;
         int ahead = 0;                                       // groups that come before this lane's
-        for (int g = 0; g < groups; g++) {
-            const double other = __shfl_sync(0xffffffffu, gs, g * lanes);
+        for (int g = 0; g < p.groups; g++) {
+            const double other = __shfl_sync(0xffffffffu, gs, g * p.lanes);
             ahead += other > gs || (other == gs && g < group);
         }
-        if (ahead >= top_groups) {
+        if (ahead >= p.top_groups) {
 #pragma unroll
             for (int i = 0; i < SLOTS; i++) key[i] = 0;
         }
@@ -110,11 +125,10 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __
             if (key[i] > best) { best = key[i]; at = i; }    // (a lane's outputs rise: ties keep the lower)
     };
     look();
-    for (int k = 0; k < top; k++) {
+    for (int k = 0; k < p.top; k++) {
         const unsigned hi = (unsigned) (best >> 32), most = __reduce_max_sync(0xffffffffu, hi);
         const unsigned lo = hi == most ? (unsigned) best : 0u, most_lo = __reduce_max_sync(0xffffffffu, lo);
-        const bool ties = hi == most && lo == most_lo;
-        const int e = ties ? first + sub + lanes * at : 0x7fffffff;
+        const int e = hi == most && lo == most_lo ? first + at : 0x7fffffff;
         const int won = __reduce_min_sync(0xffffffffu, e);
         const int from = __ffs(__ballot_sync(0xffffffffu, e == won)) - 1;
         double sc = 0.0;
@@ -127,15 +141,195 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const float * __
         sc = __shfl_sync(0xffffffffu, sc, from);
         if (lane == k) { mine = sc; mine_e = won; }
     }
-    if (renorm) {
-        double sum = lane < top ? mine : 0.0;
+    if (p.renorm) {
+        double sum = lane < p.top ? mine : 0.0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += shfl_xor_f64(sum, o);
         mine = sum == 0.0 ? 0.0 : mine / sum;
     }
-    if (lane < top) {
-        ids[t * top + lane] = mine_e;
-        wts[t * top + lane] = (float) (mine * scale);
+    if (lane < p.top) {
+        p.ids[t * p.top + lane] = mine_e;
+        p.wts[t * p.top + lane] = (float) (mine * p.scale);
+    }
+}
+
+// Descending order of a lane's keys, by Batcher's odd-even merge sort.
+template <int SLOTS> __device__ __forceinline__ void sort_keys(unsigned (&k)[SLOTS]) {
+#pragma unroll
+    for (int p = 1; p < SLOTS; p *= 2)
+#pragma unroll
+        for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+            for (int j = d % p; j + d < SLOTS; j += 2 * d)
+#pragma unroll
+                for (int i = 0; i < d; i++)
+                    if (i + j + d < SLOTS && (i + j) / (2 * p) == (i + j + d) / (2 * p)) {
+                        const unsigned x = k[i + j], y = k[i + j + d];
+                        k[i + j] = max(x, y);
+                        k[i + j + d] = min(x, y);
+                    }
+}
+
+// The same in 32 bits.  A sigmoid is off by less than 4e-7 (2 units in the last place each of the exponential and the reciprocal, which
+// matter most at 1, and the rounding of the sum between them), a softmax by less than 5e-6 of the row's largest score (the exponentials'
+// sum, 64 terms in a lane, has most of it), and the corrected score by half a unit of its own more.  Two of them whose order decides
+// anything -- neighbours among the chosen and the first that is not, the last group taken and the first that is not -- and that are nearer
+// than twice that leave the token to route_exact, as do scores that are no finite numbers.
+// Up to 8 outputs a lane, the lowest bits of a key give way to the output's slot (SLOTS units in the last place, which widen that border) and a
+// lane sorts its keys: a choice is then a reduction and a step down the winner's list, a third of the instructions of looking at all of
+// them again (8,192 tokens, 8 of 256: 17.5 us with that, bound by the integer pipe).
+template <int SLOTS>
+__global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs p, int N, int vec) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long t = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (t >= N) return;
+    const int per = p.E / p.groups, group = lane / p.lanes, j0 = (lane - group * p.lanes) * p.chunk;
+    const int first = group * per + j0, held = group < p.groups ? max(0, min(p.chunk, per - j0)) : 0;
+    const float * z = p.logits + t * p.ld + first;
+    float s[SLOTS], c[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; i++) { s[i] = -INFINITY; c[i] = 0.0f; }
+    if (vec) {                                               // whole pieces of 16 bytes
+#pragma unroll
+        for (int i = 0; i + 3 < SLOTS; i += 4)
+            if (i < held) {
+                *reinterpret_cast<float4 *>(s + i) = *reinterpret_cast<const float4 *>(z + i);
+                if (p.correction != nullptr) *reinterpret_cast<float4 *>(c + i) = __ldg(reinterpret_cast<const float4 *>(p.correction + first + i));
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++)
+            if (i < held) {
+                s[i] = z[i];
+                if (p.correction != nullptr) c[i] = __ldg(p.correction + first + i);
+            }
+    }
+    float most = 0.0f;                                       // the row's largest score, or a bound of it
+    float mx = -INFINITY;
+    if (p.softmax) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) mx = fmaxf(mx, s[i]);
+        mx = warp_max(mx);
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) {
+            s[i] = __expf(s[i] - mx);
+            sum += s[i];
+        }
+        most = __fdividef(1.0f, warp_sum(sum));
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) s[i] *= most;
+    } else {
+        most = 1.0f;
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) s[i] = route_sigmoid(s[i]);
+    }
+    constexpr bool SORT = SLOTS <= 8;
+    constexpr unsigned SLOT_BITS = SORT ? SLOTS - 1 : 0;
+    const float base = p.softmax ? 1e-5f : 2e-6f;
+    auto number = [](unsigned k) { return __int_as_float((int) (k & 0x80000000u ? k ^ 0x80000000u : ~k)); };
+    auto near_of = [&](float v) { return base * most + (base + (SORT ? SLOTS * 1.2e-7f : 0.0f)) * fabsf(v); };
+    unsigned key[SLOTS];                                     // 0: not to be chosen
+#pragma unroll
+    for (int i = 0; i < SLOTS; i++) key[i] = i < held ? (order_key(s[i] + c[i]) & ~SLOT_BITS) | (SLOT_BITS - (SORT ? i : 0)) : 0;
+    unsigned k1 = 0, k2 = 0;                                 // this lane's two largest
+    if constexpr (SORT) {
+        sort_keys<SLOTS>(key);
+        k1 = key[0];
+        k2 = key[SLOTS > 1 ? 1 : 0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) {
+            k2 = max(k2, min(k1, key[i]));
+            k1 = max(k1, key[i]);
+        }
+    }
+    bool unsure = false;
+    if (p.top_groups < p.groups) {
+        for (int o = 1; o < p.lanes; o <<= 1) {
+            const unsigned o1 = __shfl_xor_sync(0xffffffffu, k1, o), o2 = __shfl_xor_sync(0xffffffffu, k2, o);
+            k2 = max(max(k2, o2), min(k1, o1));
+            k1 = max(k1, o1);
+        }
+        const bool two = p.group_top == 2 && per > 1;
+        const float gs = two ? number(k1) + number(k2) : number(k1);
+        int ahead = 0;
+        for (int g = 0; g < p.groups; g++) {
+            const float other = __shfl_sync(0xffffffffu, gs, g * p.lanes);
+            ahead += other > gs || (other == gs && g < group);
+        }
+        const bool shut = ahead >= p.top_groups, live = group < p.groups;
+        const float lo = number(__reduce_min_sync(0xffffffffu, live && !shut ? order_key(gs) : 0xffffffffu));
+        const float hi = number(__reduce_max_sync(0xffffffffu, live && shut ? order_key(gs) : 0u));
+        // (the two that a group's score is made of may lie further from 0 than it does)
+        const float widest = two ? fmaxf(fabsf(number(k1)), fabsf(number(k2))) : fabsf(gs);
+        unsure = live && (!(widest < 1e30f) || !(lo - hi > 2.0f * near_of(widest)));
+        if (shut) {
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) key[i] = 0;
+        }
+    }
+    // The chain: a lane holds its best key; the warp's best goes to choice k, and the lane that had it leaves its output's number behind.  Equal
+    // keys, in one lane or in two, leave the token to route_exact too.
+    __shared__ int taken[4][kGroupTopMost + 1];
+    int * chosen = taken[threadIdx.x >> 5];
+    unsigned best = key[0], mine_key = 0, last_key = 0;
+    if constexpr (!SORT) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) best = max(best, key[i]);
+    }
+    for (int k = 0; k <= p.top; k++) {                       // (one more than are taken: how near it comes)
+        const unsigned won = __reduce_max_sync(0xffffffffu, best);
+        if (lane == k) mine_key = won;
+        last_key = won;                                      // (0: every output that there was is taken)
+        const unsigned who = __ballot_sync(0xffffffffu, best == won);
+        unsure = unsure || ((who & (who - 1)) != 0 && won != 0);
+        if (best == won) {
+            if constexpr (SORT) {
+                chosen[k] = first + (int) (SLOT_BITS - (won & SLOT_BITS));
+#pragma unroll
+                for (int i = 0; i + 1 < SLOTS; i++) key[i] = key[i + 1];
+                key[SLOTS - 1] = 0;
+                best = key[0];
+            } else {
+                int at = 0, equal = 0;
+                best = 0;
+#pragma unroll
+                for (int i = 0; i < SLOTS; i++) {
+                    if (key[i] == won) { key[i] = 0; at = i; equal++; }
+                    best = max(best, key[i]);
+                }
+                chosen[k] = first + at;
+                unsure = unsure || (equal > 1 && won != 0);
+            }
+        }
+    }
+    __syncwarp();
+    const float v = number(mine_key), before = __shfl_up_sync(0xffffffffu, v, 1), after = number(last_key);
+    if (lane < p.top) {
+        unsure = unsure || !(fabsf(v) < 1e30f) || (lane > 0 && !(before - v > near_of(fmaxf(fabsf(before), fabsf(v)))))
+              || (lane == p.top - 1 && last_key != 0 && !(v - after > near_of(fmaxf(fabsf(after), fabsf(v)))));
+    }
+    unsure = __any_sync(0xffffffffu, unsure);
+    const int mine_e = lane < p.top && !unsure ? chosen[lane] : 0;
+    float mine = 0.0f;
+    if (lane < p.top) {
+        const float x = p.logits[t * p.ld + mine_e];
+        mine = p.softmax ? __expf(x - mx) * most : route_sigmoid(x);
+    }
+    if (unsure) {
+        route_exact<SLOTS>(p, t);
+        return;
+    }
+    if (p.renorm) {
+        const float sum = warp_sum(lane < p.top ? mine : 0.0f);
+        mine = sum == 0.0f ? 0.0f : mine / sum;
+    }
+    if (lane < p.top) {
+        p.ids[t * p.top + lane] = mine_e;
+        p.wts[t * p.top + lane] = mine * (float) p.scale;
     }
 }
 
@@ -153,16 +347,16 @@ IIAN_API int iian_moe_route_grouped(const float * logits, long long ld, const fl
     if (E > kGroupOutputsMost || groups > kGroupsMost || top > kGroupTopMost) return IIAN_ERR_LIMIT;
     int wide = 1;
     while (wide < groups) wide *= 2;
-    const int lanes = 32 / wide, slots = (E / groups + lanes - 1) / lanes, warps = 4;
+    RouteArgs p = {logits, ld, correction, E, groups, 32 / wide, 0, top_groups, group_top, top, softmax, renorm, (double) scale, ids, wts};
+    const int per = E / groups, warps = 4;
+    p.chunk = (per + p.lanes - 1) / p.lanes;
+    const int vec = p.chunk % 4 == 0 && per % 4 == 0 && ld % 4 == 0 && (((uintptr_t) logits | (uintptr_t) correction) & 15) == 0;
     const dim3 grid((unsigned) (((long long) N + warps - 1) / warps));
-    auto go = [&](auto kernel) {
-        return iian_launch(kernel, grid, dim3(warps * 32), 0, stream, logits, ld, correction, E, groups, lanes, top_groups, group_top, top,
-                           softmax, renorm, (double) scale, ids, wts, N);
-    };
-    if (slots <= 2) return go(moe_route_grouped_kernel<2>);
-    if (slots <= 4) return go(moe_route_grouped_kernel<4>);
-    if (slots <= 8) return go(moe_route_grouped_kernel<8>);
-    if (slots <= 16) return go(moe_route_grouped_kernel<16>);
-    if (slots <= 32) return go(moe_route_grouped_kernel<32>);
+    auto go = [&](auto kernel) { return iian_launch(kernel, grid, dim3(warps * 32), 0, stream, p, N, vec); };
+    if (p.chunk <= 2) return go(moe_route_grouped_kernel<2>);
+    if (p.chunk <= 4) return go(moe_route_grouped_kernel<4>);
+    if (p.chunk <= 8) return go(moe_route_grouped_kernel<8>);
+    if (p.chunk <= 16) return go(moe_route_grouped_kernel<16>);
+    if (p.chunk <= 32) return go(moe_route_grouped_kernel<32>);
     return go(moe_route_grouped_kernel<64>);                 // 17 groups of 60: half of the lanes hold nothing
 }
