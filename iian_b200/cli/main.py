@@ -1,4 +1,4 @@
-"""``iian <command>``: complete, bench, random-weights, version.
+"""``iian <command>``: complete, score, bench, random-weights, version.
 
 Commands, option names and meanings follow the reference's command line where it has them
 (src/iian/cli/commands.cpp:15-34; ``complete``: src/iian/cli/cmd_run.cpp:225-256; ``bench``:
@@ -15,7 +15,7 @@ from typing import List, Optional
 
 from .args import Options
 
-COMMANDS = ("complete", "bench", "random-weights", "version")
+COMMANDS = ("complete", "score", "bench", "random-weights", "version")
 
 
 def _add_engine_flags(o: Options) -> None:
@@ -128,6 +128,38 @@ def cmd_complete(argv: List[str]) -> int:
                          indent=2))
     else:
         print(" ".join(str(t) for t in toks))
+    return 0
+
+
+def cmd_score(argv: List[str]) -> int:
+    o = Options("iian score", "Natural log-probabilities of given token ids, each given those before it (nothing is generated).")
+    o.positional("model", "model folder (config.json + model.safetensors)")
+    o.add("-p,--prompt", "Token ids, e.g. '1,2,3'; several sequences separated by ';' ('-' reads them from stdin, a sequence a line)", "IDS")
+    o.add("--start", "First place whose token is scored (1 = the second token; a place behind the prompt scores an answer alone)", "N", 1, int)
+    o.flag("--json", "Print a JSON object per sequence with every log-probability, their sum and the perplexity")
+    _add_engine_flags(o)
+    ns = o.parse(argv)
+    import math
+    from ..engine.engine import Engine
+    try:
+        if not ns.prompt:
+            print("iian score: missing -p/--prompt (token ids)", file=sys.stderr)
+            return 1
+        lines = sys.stdin.read().splitlines() if ns.prompt == "-" else ns.prompt.split(";")
+        seqs = [ids for ids in (_parse_ids(line) for line in lines) if ids]
+        engine = Engine(ns.model, engine_config_from_args(ns))
+        scores = engine.score(seqs, [ns.start] * len(seqs))
+    except (ValueError, FileNotFoundError, KeyError, RuntimeError) as e:
+        print(f"iian score: {e}", file=sys.stderr)
+        return 1
+    for ids, lp in zip(seqs, scores):
+        total = math.fsum(lp)
+        mean = -total / len(lp) if lp else 0.0
+        ppl = math.exp(mean) if mean < 700.0 else math.inf
+        if ns.json:
+            print(json.dumps({"tokens": ids, "start": ns.start, "logprobs": lp, "sum": total, "perplexity": ppl}))
+        else:
+            print(f"{len(lp)} tokens  log-probability {total:.6f}  perplexity {ppl:.6f}")
     return 0
 
 
@@ -270,6 +302,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     argv = list(sys.argv[1:] if argv is None else argv)
     if not argv or argv[0] in ("-h", "--help"):
         print("usage: iian <command> [options]\n\ncommands:\n  complete        generate from a prompt of token ids\n"
+              "  score           log-probabilities of given token ids\n"
               "  bench           throughput at several concurrency levels\n  random-weights  write a model folder with random weights\n"
               "  version         print the version\n\n'iian <command> --help' lists a command's options.")
         return 0
@@ -280,6 +313,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         return 0
     if cmd == "complete":
         return cmd_complete(rest)
+    if cmd == "score":
+        return cmd_score(rest)
     if cmd == "bench":
         return cmd_bench(rest)
     if cmd == "random-weights":

@@ -29,7 +29,7 @@ template <int ACT> __device__ __forceinline__ float linear_act_of(float y) {
         const float x = 0.7071067811865476f * fabsf(y);
         float d = fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, 0.0000430638f, 0.0002765672f), 0.0001520143f), 0.0092705272f), 0.0422820123f), 0.0705230784f), 1.0f);
         d *= d; d *= d; d *= d;
-        return fmaf(-0.5f * fabsf(y), linear_rcp(d * d), y < 0.0f ? 0.0f : y);
+        return fmaf(-0.5f * fminf(fabsf(y), 64.0f), linear_rcp(d * d), y < 0.0f ? 0.0f : y);        // (an infinity times the 0 there would be no number)
     } else if constexpr (ACT == LACT_RELU) return y < 0.0f ? 0.0f : y;        // (what is no number stays none)
     else if constexpr (ACT == LACT_RELU2) return y < 0.0f ? 0.0f : y * y;
     else return y;

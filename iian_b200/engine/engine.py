@@ -5,7 +5,8 @@ src/iian/engine.cpp): ``submit`` validates and queues a tokenized prompt (engine
 ``step`` schedules, runs one mixed batch, advances the computed counts, samples one token for every
 request whose last token was in the batch, applies the stop rules and frees finished requests
 (engine.cpp:456-637, :639-762); ``generate`` submits and steps until everything is finished.
-Text, logprobs, grammars, embeddings and speculative decoding are not part of this engine.
+``score`` runs given token ids through the same step function and says how likely each is.
+Text, grammars, embeddings and speculative decoding are not part of this engine.
 
 Sizing (engine.cpp:105, :131-165): ``max_model_len`` defaults to min(the model's positions, 8192);
 the cache holds ``max_model_len * min(max_num_seqs, 4)`` tokens unless told otherwise, capped by
@@ -295,6 +296,80 @@ class Engine:
             if r.finish_reason == FinishReason.ERROR:
                 raise RuntimeError(f"request {r.id}: {r.error}")
         return [r.output_tokens for r in reqs]
+
+    def score(self, sequences: Sequence[Sequence[int]], starts: Optional[Sequence[int]] = None) -> List[List[float]]:
+        """Natural log-probability of every token of each sequence given those before it, from place ``starts[i]`` on (default 1: all that
+        have one before them).  Nothing is generated and no logits are kept: a prompt of any length costs two numbers a token.
+
+        Sequences run through the step function in portions of ``max_num_batched_tokens``, several at a time, beside the pages that
+        requests under way hold; where they do not fit together the later ones wait.  Not while the background loop runs."""
+        if self._thread is not None:
+            raise RuntimeError("score: the background loop is running; stop() it first")
+        seqs = [[int(t) for t in s] for s in sequences]
+        first = [1] * len(seqs) if starts is None else [int(s) for s in starts]
+        if len(first) != len(seqs):
+            raise ValueError(f"score: {len(first)} starts for {len(seqs)} sequences")
+        for s, at in zip(seqs, first):
+            if not s:
+                raise ValueError("score: a sequence must not be empty")
+            if at < 1:
+                raise ValueError(f"score: there is nothing before place {at - 1} to predict it from (starts are 1 or more)")
+            if len(s) > self.max_model_len:
+                raise ValueError(f"score: a sequence of {len(s)} tokens, max_model_len is {self.max_model_len}")
+            for t in s:
+                if t < 0 or t >= self.model.vocab_size:
+                    raise ValueError(f"score: token id out of range: {t}")
+        out: List[List[float]] = [[] for _ in seqs]
+        waiting = [i for i, s in enumerate(seqs) if len(s) > first[i]]
+        live: List[list] = []                 # [sequence, its cache, tokens done], oldest first
+        mgr, budget = self.cache, self.cfg.sched.max_num_batched_tokens
+        try:
+            while waiting or live:
+                while waiting and len(live) < self.runner.max_num_seqs:
+                    rc = mgr.new_request()
+                    if not mgr.allot_state(rc):
+                        break
+                    live.append([waiting.pop(0), rc, 0])
+                if not live:
+                    raise RuntimeError("score: requests under way hold every state slot")
+                entries, targets, moved, left = [], [], [], budget
+                for k, (i, rc, done) in enumerate(live):
+                    n = min(left, len(seqs[i]) - 1 - done)          # the last token predicts nothing
+                    if n == 0:
+                        break
+                    mgr.release_passed(rc, done)
+                    if not mgr.allocate(rc, done, n):
+                        # those behind it give their pages back and begin again later; alone it cannot go on
+                        if k == 0 and len(live) == 1:
+                            raise RuntimeError(f"score: a sequence of {len(seqs[i])} tokens does not fit in the KV cache")
+                        for j, c, _ in reversed(live[max(k, 1):]):
+                            mgr.free(c)
+                            out[j] = []
+                            waiting.insert(0, j)
+                        del live[max(k, 1):]
+                        break
+                    want = range(max(0, first[i] - 1 - done), n)
+                    entries.append(StepEntry(rc, seqs[i][done: done + n], done, want))
+                    targets.append([seqs[i][done + j + 1] for j in want])
+                    moved.append((live[k], n))
+                    left -= n
+                if not entries:
+                    continue                    # the oldest one has the pages to itself now
+                got = self.runner.score(entries, targets)
+                values = got[0].tolist() if got is not None else []
+                self.runner.check_device_status()
+                at = 0
+                for (item, n), t in zip(moved, targets):
+                    out[item[0]].extend(values[at: at + len(t)])
+                    at += len(t)
+                    item[2] += n
+                for item in [m for m, _ in moved if m[2] == len(seqs[m[0]]) - 1]:
+                    live.remove(item)
+                    mgr.free(item[1])
+        finally:
+            for item in live:
+                mgr.free(item[1])
+        return out
 
     def warmup(self) -> None:
         """A small prefill and two decode steps, so that kernels are compiled and loaded before the

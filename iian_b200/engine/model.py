@@ -180,18 +180,19 @@ class Model:
         return sorted(libs)
 
     # ---- one step ----------------------------------------------------------------------------
-    def forward(self, ctx, storage) -> Optional[torch.Tensor]:
+    def forward(self, ctx, storage, targets: Optional[torch.Tensor] = None):
         """Run ``ctx.tokens`` through the model and return float32 logits ``[R, vocab]`` for
-        ``ctx.out_rows`` (None if no row is wanted; the caches are still updated)."""
+        ``ctx.out_rows`` (None if no row is wanted; the caches are still updated).  With ``targets`` (int32 [R]) no logits are formed:
+        what comes back are the targets' log-probabilities and the rows' log-sum-exps, float32 [R] each."""
         if hasattr(ctx, "step_cache"):
             ctx.step_cache.clear()          # a context may be run twice (eagerly, then under graph capture)
         if self.device.type == "cuda":
             from ..ops.cuda_backend import pin_stream
             with pin_stream():
-                return self._forward(ctx, storage)
-        return self._forward(ctx, storage)
+                return self._forward(ctx, storage, targets)
+        return self._forward(ctx, storage, targets)
 
-    def _forward(self, ctx, storage) -> Optional[torch.Tensor]:
+    def _forward(self, ctx, storage, targets: Optional[torch.Tensor] = None):
         residual = self.embedding.forward(ctx.tokens, ctx)
         delta = None
         order = self.spec.order
@@ -226,4 +227,4 @@ class Model:
         if ctx.out_rows.shape[0] == 0:
             return None
         normed = self.final_norm.forward(residual, delta, ctx)
-        return self.head.forward(normed, ctx)
+        return self.head.forward(normed, ctx) if targets is None else self.head.score(normed, targets, ctx)

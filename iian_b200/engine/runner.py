@@ -472,6 +472,27 @@ class ModelRunner:
         self.last_upload_bytes = ctx.upload_bytes
         return out
 
+    def score(self, entries: Sequence[StepEntry], targets: Sequence[Sequence[int]]):
+        """A step that says how likely given tokens are instead of returning logits: ``targets[i][j]`` is the token asked about at place
+        ``entries[i].want[j]`` (negative: none).  Returns their log-probabilities and the places' log-sum-exps, float32 tensors in the
+        order of the entries and of their ``want`` lists, valid until the next step (None if nothing is wanted)."""
+        if not entries:
+            return None
+        if len(entries) > self.max_num_seqs:
+            raise ValueError(f"{len(entries)} requests in one step, the runner was built for {self.max_num_seqs}")
+        if len(targets) != len(entries) or any(len(t) != len(e.want) for t, e in zip(targets, entries)):
+            raise ValueError("score: a token for every wanted place")
+        flat = [int(t) for row in targets for t in row]
+        if any(t >= self.model.vocab_size for t in flat):
+            raise ValueError(f"score: a token outside the vocabulary ({self.model.vocab_size})")
+        ctx = self.build_context(entries)
+        want = torch.tensor(flat, dtype=torch.int32).to(self.device)
+        before = _launch_count()
+        out = self.model.forward(ctx, self.storage, want)
+        self.launches += _launch_count() - before
+        self.last_upload_bytes = ctx.upload_bytes + 4 * len(flat)
+        return out
+
     # ---- decode-only steps replayed from captured CUDA graphs ------------------------------------
     def _step_graph(self, entries: Sequence[StepEntry]) -> torch.Tensor:
         """The reference replays whole steps from CUDA graphs keyed by the batch's shape

@@ -236,6 +236,7 @@ class Mixer(Part):
 
 class FeedForward(Part):
     folds_norm_out = False
+    adds_residual = False        # forward(x, ctx, residual=r) adds the output into the float32 stream r and returns None
 
     def takes_prenormed(self, n_rows: int) -> bool:
         return False
@@ -256,6 +257,10 @@ class Embedding(Part):
 class Head(Part):
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:  # pragma: no cover
         raise NotImplementedError
+
+    def score(self, x: torch.Tensor, targets: torch.Tensor, ctx):
+        """(log-probabilities of given tokens, log-sum-exps) of the rows; a head that can say no more than its logits does not have it."""
+        raise NotImplementedError(f"{type(self).__name__} gives logits only")
 
 
 class StreamPart(Part):

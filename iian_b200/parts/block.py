@@ -89,6 +89,8 @@ class PreNormResidualBlock:
             k.gather_rows(y, select_rows, y_sel)
             residual, y = res_sel, y_sel
         h2 = y if isinstance(y, Prenormed) else self.feed_forward_norm.forward(residual, y, ctx)
+        if self.feed_forward.adds_residual:
+            return residual, self.feed_forward.forward(h2, ctx, residual=residual)        # (None: nothing is owed to the stream)
         request = None
         if self.feed_forward.folds_norm_out:
             request = self._norm_out(next_norm, next_consumer, residual, residual.shape[0], "feed_forward")

@@ -118,3 +118,11 @@ class LMHead(Head):
         if self.softcap is not None:
             ops.kernels().tanh_cap(logits, self.softcap)
         return logits
+
+    def score(self, x: torch.Tensor, targets: torch.Tensor, ctx):
+        """Log-probability of row r's token ``targets[r]`` (int32; negative: none, 0) and the row's log-sum-exp, float32 [R] each, without
+        the logits."""
+        lp = ctx.buf("score_logprobs", (x.shape[0],), torch.float32)
+        lse = ctx.buf("score_lse", (x.shape[0],), torch.float32)
+        ops.kernels().linear_logprobs(x, self.weight, targets, lp, lse, softcap=self.softcap)
+        return lp, lse

@@ -29,6 +29,12 @@ the input instead.  ``activation = "relu2"``: experts without a gate, ``Wdown ma
 ``shared_gate``: the shared expert's output is multiplied by ``sigmoid(w h)``, one number per token; its row ``shared.sg``
 rides under the router's in the product with float32 output.
 
+``score = "grouped"``: scores ``s = sigmoid(z)`` or ``softmax(z)`` (``score_function``), ``c = s + correction`` (a tensor of one number an
+expert, for the choice alone; ``correction`` false: none).  The experts come in ``groups`` groups of neighbours, a group's score is the
+sum of its ``group_top`` (1 or 2) largest ``c``; of the ``top_groups`` best groups a token takes the ``top`` experts with the largest ``c``, and
+each weighs ``weight_scale * s``, divided by the sum of the chosen ``s`` unless ``renormalise`` is false; ``shared_gate`` may scale the shared
+expert by a sigmoid of its own.
+
 ``stack_rows`` puts further rows that read the same input (a gate of the residual) under the router's, so that one
 product with float32 output serves both.
 """
@@ -47,7 +53,8 @@ from .base import FeedForward, register_feed_forward
 class RoutedExperts(FeedForward):
     """params: ``hidden_size``, ``num_experts``, ``top``, ``intermediate_size`` (of one expert), ``activation``
     (``silu`` | ``gelu_tanh`` | ``clamped_swish`` with ``limit`` | ``relu2``), ``score`` (``sigmoid`` | ``softmax_top`` with
-    ``router_bias`` | ``softmax`` with ``weight_scale`` and ``identity_experts`` | ``table`` with ``vocab_size``), ``weight_on`` (``input`` | ``output``),
+    ``router_bias`` | ``softmax`` with ``weight_scale`` and ``identity_experts`` | ``grouped`` with ``score_function``, ``groups``, ``top_groups``,
+    ``group_top``, ``correction``, ``renormalise`` and ``weight_scale`` | ``table`` with ``vocab_size``), ``weight_on`` (``input`` | ``output``),
     ``shared_intermediate_size`` with ``shared_gate`` and ``shared_limit``."""
 
     SWISH_ALPHA = 1.702         # fixed by the clamped activation (also in the kernels)
@@ -67,14 +74,27 @@ class RoutedExperts(FeedForward):
             raise ValueError("routed_experts: the clamped activation needs a positive limit")
         self.score = p.get("score", "sigmoid")
         self.weight_on = p.get("weight_on", "input")
-        if self.score not in ("sigmoid", "softmax_top", "softmax", "table") or self.weight_on not in ("input", "output"):
-            raise ValueError("routed_experts: score is 'sigmoid', 'softmax_top', 'softmax' or 'table', weight_on 'input' or 'output'")
+        if self.score not in ("sigmoid", "softmax_top", "softmax", "grouped", "table") or self.weight_on not in ("input", "output"):
+            raise ValueError("routed_experts: score is 'sigmoid', 'softmax_top', 'softmax', 'grouped' or 'table', weight_on 'input' or 'output'")
         self.identity = int(p.get("identity_experts", 0) or 0)
         self.weight_scale = float(p.get("weight_scale", 1.0))
-        if (self.identity or self.weight_scale != 1.0) and self.score != "softmax":
-            raise ValueError("routed_experts: identity_experts and weight_scale come with score 'softmax'")
-        if self.score == "softmax" and self.weight_on != "output":
-            raise ValueError("routed_experts: with score 'softmax' the weight is on the output")
+        if (self.identity and self.score != "softmax") or (self.weight_scale != 1.0 and self.score not in ("softmax", "grouped")):
+            raise ValueError("routed_experts: identity_experts and weight_scale come with score 'softmax' (weight_scale with 'grouped' too)")
+        if self.score in ("softmax", "grouped") and self.weight_on != "output":
+            raise ValueError(f"routed_experts: with score '{self.score}' the weight is on the output")
+        self.score_function = p.get("score_function", "sigmoid")
+        self.groups, self.top_groups = int(p.get("groups", 1)), int(p.get("top_groups", 1))
+        self.group_top, self.renormalise = int(p.get("group_top", 2)), bool(p.get("renormalise", True))
+        self.has_correction = self.score == "softmax" or (self.score == "grouped" and bool(p.get("correction", True)))
+        if self.score == "grouped":
+            if self.score_function not in ("sigmoid", "softmax"):
+                raise ValueError(f"routed_experts: score_function is 'sigmoid' or 'softmax', not {self.score_function!r}")
+            if self.groups < 1 or self.experts % self.groups or not 1 <= self.top_groups <= self.groups or self.group_top not in (1, 2) \
+                    or self.top > self.top_groups * (self.experts // self.groups):
+                raise ValueError(f"routed_experts: {self.top} of {self.experts} experts, {self.top_groups} of {self.groups} groups known by "
+                                 f"their best {self.group_top}")
+            if self.experts > 1024 or self.groups > 32 or self.top > 32:
+                raise ValueError("routed_experts: grouped choice goes up to 1,024 experts, 32 groups and 32 experts a token")
         self.outputs = self.experts + self.identity         # of the router
         self.correction = None
         self.shared_inter = int(p.get("shared_intermediate_size", 0) or 0)
@@ -92,8 +112,8 @@ class RoutedExperts(FeedForward):
                                                               "limit": float(p.get("shared_limit", self.limit)),
                                                               "names": ("shared.gate", "shared.up", "shared.down")}), dtype, device)
         self.shared_gate = bool(p.get("shared_gate", False)) and self.shared is not None
-        if self.shared_gate and self.score not in ("softmax", "softmax_top"):
-            raise ValueError("routed_experts: shared_gate comes with score 'softmax' or 'softmax_top'")
+        if self.shared_gate and self.score not in ("softmax", "softmax_top", "grouped"):
+            raise ValueError("routed_experts: shared_gate comes with score 'softmax', 'softmax_top' or 'grouped'")
         self.has_router_bias = self.score == "softmax_top" and bool(p.get("router_bias", True))
         self.router_bias = None
         self.vocab = int(p["vocab_size"]) if self.score == "table" else 0
@@ -109,7 +129,7 @@ class RoutedExperts(FeedForward):
             t = {"table": TensorSpec((self.vocab, self.top), kind="int", init=f"distinct_rows:{self.experts}")}
         else:
             t = {"router": TensorSpec((self.outputs, self.hidden))}
-            if self.score == "softmax":
+            if self.has_correction:
                 t["correction"] = TensorSpec((self.outputs,), init="zeros_jitter")
             if self.shared_gate:
                 t["shared.sg"] = TensorSpec((1, self.hidden))
@@ -132,7 +152,7 @@ class RoutedExperts(FeedForward):
             self.w_router = self._router.contiguous()
             if self.has_router_bias:
                 self.router_bias = tensors["router.b"].to(torch.float32).contiguous()
-            if self.score == "softmax":
+            if self.has_correction:
                 self.correction = tensors["correction"].to(torch.float32).contiguous()
             if self.shared_gate:
                 self.stack_rows(tensors["shared.sg"])
@@ -163,9 +183,10 @@ class RoutedExperts(FeedForward):
         self.w_router = torch.cat(ws, dim=0).contiguous()
 
     def kernel_libraries(self):
+        own = ("moe", "gemm_simt") + (("moe_groups",) if self.score == "grouped" else ())
         if self.shared is not None:
-            return tuple(set(("moe", "gemm_simt") + tuple(self.shared.kernel_libraries())))
-        return ("moe", "gemm_simt")        # in bfloat16 the products' fast forms come with gemm_simt (the grouped tcgen05 one too)
+            return tuple(set(own + tuple(self.shared.kernel_libraries())))
+        return own        # in bfloat16 the products' fast forms come with gemm_simt (the grouped tcgen05 one too)
 
     def forward(self, x, ctx, with_extra: bool = False, rows=None):
         """``rows`` (int32, optional): the step's token each row of ``x`` belongs to, when ``x`` holds selected rows only
@@ -187,6 +208,9 @@ class RoutedExperts(FeedForward):
             k.linear(x, self.w_router, logits)
             if self.score == "softmax":
                 k.moe_route_corrected(logits[:, : self.outputs], self.correction, top, ids, wts, self.weight_scale)
+            elif self.score == "grouped":
+                k.moe_route_grouped(logits[:, :E], top, ids, wts, score=self.score_function, correction=self.correction, groups=self.groups,
+                                    top_groups=self.top_groups, group_top=self.group_top, renormalise=self.renormalise, scale=self.weight_scale)
             elif self.score == "softmax_top":
                 k.moe_route_softmax(logits[:, :E], self.router_bias, top, ids, wts)
             else:

@@ -138,24 +138,41 @@ class PlainMLP(FeedForward):
     """A feed-forward without a gate: ``y = Wdown act(Wup h)``.
 
     params: ``hidden_size``, ``intermediate_size``, ``activation``: ``xielu`` (two learned numbers p, q in a tensor of
-    their own: ``z > 0: softplus(p) z^2 + z / 2``, else ``(1/2 + softplus(q)) (exp(z) - 1 - z) + z / 2``) or ``relu2``
-    (``max(z, 0)^2``, no tensor); optional ``names``: the local tensor names of (up, down, the activation's numbers)."""
+    their own: ``z > 0: softplus(p) z^2 + z / 2``, else ``(1/2 + softplus(q)) (exp(z) - 1 - z) + z / 2``), ``relu2``
+    (``max(z, 0)^2``), ``silu``, ``gelu`` (by erf), ``gelu_tanh`` or ``relu``; optional ``bias`` (default false): ``y = Wdown act(Wup h + b1) +
+    b2``; optional ``names``: the local tensor names of (up, down, the activation's numbers[, up's bias, down's bias]).
+
+    ``silu``, ``gelu``, ``gelu_tanh``, ``relu`` and every form with biases run as two products with bias and activation in their epilogues, and
+    the second may add into the float32 stream itself (``adds_residual``), unrounded in between; ``xielu`` and ``relu2`` without biases
+    as product, activation kernel, product."""
+
+    FUSED = ("silu", "gelu", "gelu_tanh", "relu")
 
     def __init__(self, spec, dtype, device):
         super().__init__(spec, dtype, device)
         self.hidden = int(spec["hidden_size"])
         self.inter = int(spec["intermediate_size"])
         act = spec.params.get("activation", "xielu")
-        if act not in ("xielu", "relu2"):
-            raise ValueError(f"plain_mlp: activation '{act}' has no kernel (xielu, relu2)")
+        if act not in ("xielu", "relu2") + self.FUSED:
+            raise ValueError(f"plain_mlp: activation '{act}' has no kernel (xielu, relu2, {', '.join(self.FUSED)})")
         self.activation = act
+        self.bias = bool(spec.params.get("bias", False))
+        if self.bias and act == "xielu":
+            raise ValueError("plain_mlp: xielu has no form with biases")
+        self.fused = self.bias or act in self.FUSED
+        self.adds_residual = self.fused
         self.names = tuple(spec.params.get("names", ("up", "down", "act")))
-        self.w_up = self.w_down = self.act_numbers = None
+        if self.bias and len(self.names) < 5:
+            self.names = (self.names + ("act",))[:3] + ("up.b", "down.b")
+        self.w_up = self.w_down = self.act_numbers = self.b_up = self.b_down = None
 
     def tensors(self) -> Dict[str, TensorSpec]:
         t = {self.names[0]: TensorSpec((self.inter, self.hidden)), self.names[1]: TensorSpec((self.hidden, self.inter))}
         if self.activation == "xielu":
             t[self.names[2]] = TensorSpec((2,), init="zeros_jitter")
+        if self.bias:
+            t[self.names[3]] = TensorSpec((self.inter,))
+            t[self.names[4]] = TensorSpec((self.hidden,))
         return t
 
     def bind(self, tensors: Dict[str, torch.Tensor]) -> None:
@@ -163,13 +180,28 @@ class PlainMLP(FeedForward):
         self.w_down = tensors[self.names[1]].contiguous()
         if self.activation == "xielu":
             self.act_numbers = tensors[self.names[2]].to(torch.float32).contiguous()
+        if self.bias:
+            self.b_up = tensors[self.names[3]].to(torch.float32).contiguous()
+            self.b_down = tensors[self.names[4]].to(torch.float32).contiguous()
 
     def kernel_libraries(self):
+        if self.fused:
+            return ("linear_fused", "gemm_simt")
         return ("residual_ops", "gemm_simt")
 
-    def forward(self, x, ctx):
+    def forward(self, x, ctx, residual=None):
+        """With ``residual`` (float32 [N, hidden]; only where ``adds_residual``) the output is added into it and None returned."""
         k = ops.kernels()
         n = x.shape[0]
+        if self.fused:
+            act = ctx.buf("ffn_act", (n, self.inter), self.dtype)
+            k.linear_act(x, self.w_up, act, bias=self.b_up, activation=self.activation)
+            if residual is not None:
+                k.linear_act(act, self.w_down, residual, bias=self.b_down, residual=residual)
+                return None
+            out = ctx.buf("ffn_out", (n, self.hidden), self.dtype)
+            k.linear_act(act, self.w_down, out, bias=self.b_down)
+            return out
         up = ctx.buf("ffn_up", (n, self.inter), self.dtype)
         k.linear(x, self.w_up, up)
         act = ctx.buf("ffn_act", (n, self.inter), self.dtype)
