@@ -20,30 +20,31 @@ namespace iian {
 
 constexpr int BM = 64, BN = 64, BK = 16;
 
-// What becomes of a sum, and how far apart the rows of x are: the product itself ...
-template <typename TO>
-struct PlainOut {
-    TO * out;
-    int M;
-    __device__ __forceinline__ void operator()(int n, int m, float v) const { out[(size_t) n * M + m] = from_f32<TO>(v); }
-    __device__ __forceinline__ size_t ldx(int K) const { return (size_t) K; }
-};
-// ... or with bias, activation and residual (epilogue.cuh)
-struct FusedOut {
+// What becomes of a sum, and how far apart the rows of x are: the product itself goes to `out` ...
+struct Plain { static constexpr bool fused = false; };
+// ... or with bias, activation and residual (epilogue.cuh) to where that says
+struct Fused {
+    static constexpr bool fused = true;
     LinearEpilogue e;
-    long long ld;
-    __device__ __forceinline__ void operator()(int n, int m, float v) const { e.store(v, (size_t) n, m); }
-    __device__ __forceinline__ size_t ldx(int) const { return (size_t) ld; }
+    int ldx;
 };
+template <typename EPI> __device__ __forceinline__ int row_distance(const EPI & epi, int K) {
+    if constexpr (EPI::fused) return epi.ldx;
+    else return K;
+}
+template <typename TO, typename EPI> __device__ __forceinline__ void put_out(TO * __restrict__ out, const EPI & epi, int n, int m, int M, float v) {
+    if constexpr (EPI::fused) epi.e.store(v, (size_t) n, m);
+    else out[(size_t) n * M + m] = from_f32<TO>(v);
+}
 
-template <typename TX, typename TW, typename OUT>
+template <typename TX, typename TW, typename TO, typename EPI>
 __global__ void __launch_bounds__(256) gemm_simt_kernel(const TX * __restrict__ x, const TW * __restrict__ w,
-                                                        const OUT out, int N, int M, int K) {
+                                                        TO * __restrict__ out, int N, int M, int K, const EPI epi) {
     __shared__ float xs[BK][BN + 4];
     __shared__ float ws[BK][BM + 4];
     const int tid = threadIdx.x;
     const int n0 = blockIdx.y * BN, m0 = blockIdx.x * BM;
-    const size_t ldx = out.ldx(K);
+    const int ldx = row_distance(epi, K);
     const int tx = tid % 16, ty = tid / 16;          // thread computes rows n0 + ty*4.., cols m0 + tx*4..
     const int lrow = tid / 4, lk = (tid % 4) * 4;    // loader: row of the tile, first k of 4
     float acc[4][4];
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const TX * __restrict__ 
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int m = m0 + tx * 4 + j;
-            if (m < M) out(n, m, acc[i][j]);
+            if (m < M) put_out(out, epi, n, m, M, acc[i][j]);
         }
     }
 }
@@ -94,9 +95,9 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const TX * __restrict__ 
 // multiply-adds).  The loader's 16-byte pieces along k are put down as four words in four rows, the column flipped by 8 in the upper
 // half of a stage so that a warp's words fall into 32 banks.  2,048 x 6,144 x 4,096: 2,023 us (51 TFLOP/s; 4 x 4 blocks without
 // packing 3,996 us).
-template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename OUT>
+template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO, typename EPI>
 __global__ void __launch_bounds__((TILE_N / TN) * (TILE_M / TM))
-gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, const OUT out, int N, int M, int K) {
+gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
     constexpr int THREADS = (TILE_N / TN) * (TILE_M / TM), TX = TILE_M / TM;
     constexpr int LX = TILE_N * BK / 4 / THREADS, LW = TILE_M * BK / 4 / THREADS;        // 16-byte pieces a thread loads per stage
     static_assert(LX * THREADS * 4 == TILE_N * BK && LW * THREADS * 4 == TILE_M * BK && BK == 16, "whole pieces per thread");
@@ -104,7 +105,7 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, con
     __shared__ __align__(16) float ws[2][BK][TILE_M + 4];
     const int tid = threadIdx.x, tx = tid % TX, ty = tid / TX;
     const int n0 = blockIdx.y * TILE_N, m0 = blockIdx.x * TILE_M;
-    const size_t ldx = out.ldx(K);
+    const int ldx = row_distance(epi, K);
     unsigned long long acc[TN][TM / 2];
 #pragma unroll
     for (int i = 0; i < TN; i++)
@@ -183,8 +184,8 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, con
         for (int j = 0; j < TM / 2; j++) {
             const int m = m0 + (j / 2) * (TILE_M / (TM / 4)) + tx * 4 + (j % 2) * 2;
             const float2 v = unpack2(acc[i][j]);
-            if (m < M) out(n, m, v.x);
-            if (m + 1 < M) out(n, m + 1, v.y);
+            if (m < M) put_out(out, epi, n, m, M, v.x);
+            if (m + 1 < M) put_out(out, epi, n, m + 1, M, v.y);
         }
     }
 }
@@ -195,16 +196,16 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, con
 // Lanes are dealt so that neighbours share a row of one operand or of the other (bits 0 and 4 pick the row of x, bits 1 to 3 that of w):
 // 16-byte reads then take 2 clocks a warp, 4 where equal addresses lie 8 lanes apart.  What bounds it: one warp a scheduler leaves
 // the 4-clock chain and the reads' latency bare, more of them the dispatch of three-operand multiply-adds (41 clocks for 32).
-template <int TN, int TM, int WY, int WX, int STAGES, int DEPTH, typename OUT>
+template <int TN, int TM, int WY, int WX, int STAGES, int DEPTH, typename TO, typename EPI>
 __global__ void __launch_bounds__(WY * WX * 32)
-gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, const OUT out, int N, int M, int K) {
+gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
     constexpr int TILE_N = 4 * TN * WY, TILE_M = 8 * TM * WX, THREADS = WY * WX * 32, LD = DEPTH + 4, PIECES = DEPTH / 4;
     constexpr int LOADS = (TILE_N + TILE_M) * PIECES / THREADS;
     static_assert(LOADS * THREADS == (TILE_N + TILE_M) * PIECES && THREADS % PIECES == 0, "whole pieces per thread");
     extern __shared__ __align__(16) float ring[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n0 = blockIdx.y * TILE_N, m0 = blockIdx.x * TILE_M;
-    const size_t ldx = out.ldx(K);
+    const int ldx = row_distance(epi, K);
     const int turns = (K + DEPTH - 1) / DEPTH;
     auto fill = [&](int s) {
         if (s < turns) {
@@ -216,7 +217,7 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, con
                 const bool is_x = r < TILE_N;
                 const int g = is_x ? n0 + r : m0 + r - TILE_N;
                 const bool in = k < K && g < (is_x ? N : M);
-                copy16(to + r * LD, in ? (is_x ? x + (size_t) g * ldx : w + (size_t) g * K) + k : x, in);
+                copy16(to + r * LD, in ? (is_x ? x : w) + (size_t) g * (is_x ? ldx : K) + k : x, in);
             }
         }
         asm volatile("cp.async.commit_group;");
@@ -267,7 +268,7 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, con
 #pragma unroll
         for (int j = 0; j < TM; j++) {
             const int m = m0 + col + 8 * j;
-            if (m < M) out(n, m, acc[i][j]);
+            if (m < M) put_out(out, epi, n, m, M, acc[i][j]);
         }
     }
 }
@@ -279,13 +280,13 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, con
 // 2 x 1,024 x 3,072: 20 us (210 us).
 constexpr int kRowsThreads = 128, kRowsK = 128, kRowsMax = 16;
 
-template <int TILE_M, int STAGES, int PER, typename OUT>
+template <int TILE_M, int STAGES, int PER, typename TO, typename EPI>
 __global__ void __launch_bounds__(kRowsThreads)
-gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, const OUT out, int N, int M, int K) {
+gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
     constexpr int LD = kRowsK + 4, GROUPS = kRowsThreads / TILE_M;       // rows 4 banks apart: 16-byte reads of 8 lanes hit 32 banks
     extern __shared__ __align__(16) float ring[];
     const int stage_floats = (TILE_M + N) * LD;
-    const size_t ldx = out.ldx(K);
+    const int ldx = row_distance(epi, K);
     const int tid = threadIdx.x, m0 = blockIdx.x * TILE_M, m = tid % TILE_M, g = tid / TILE_M;
     const int turns = (K + kRowsK - 1) / kRowsK;
     auto fill = [&](int s) {
@@ -332,38 +333,38 @@ gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, con
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int n = g + i * GROUPS;
-        if (n < N && m0 + m < M) out(n, m0 + m, acc[i]);
+        if (n < N && m0 + m < M) put_out(out, epi, n, m0 + m, M, acc[i]);
     }
 }
 
-template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename OUT>
-static int launch_tile(const float * x, const float * w, const OUT & out, int N, int M, int K, cudaStream_t stream) {
+template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO, typename EPI>
+static int launch_tile(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
     const dim3 grid((M + TILE_M - 1) / TILE_M, (N + TILE_N - 1) / TILE_N);
-    gemm_tile_kernel<TILE_N, TILE_M, TN, TM, AHEAD, OUT><<<grid, (TILE_N / TN) * (TILE_M / TM), 0, stream>>>(x, w, out, N, M, K);
+    gemm_tile_kernel<TILE_N, TILE_M, TN, TM, AHEAD, TO, EPI><<<grid, (TILE_N / TN) * (TILE_M / TM), 0, stream>>>(x, w, out, N, M, K, epi);
     return iian_launch_status();
 }
 
-template <int TN, int TM, int STAGES, int DEPTH, typename OUT>
-static int launch_ring(const float * x, const float * w, const OUT & out, int N, int M, int K, cudaStream_t stream) {
+template <int TN, int TM, int STAGES, int DEPTH, typename TO, typename EPI>
+static int launch_ring(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
     constexpr int TILE_N = 8 * TN, TILE_M = 16 * TM;         // two by two warps
     constexpr size_t smem = (size_t) STAGES * (TILE_N + TILE_M) * (DEPTH + 4) * sizeof(float);
-    auto kernel = gemm_ring_kernel<TN, TM, 2, 2, STAGES, DEPTH, OUT>;
+    auto kernel = gemm_ring_kernel<TN, TM, 2, 2, STAGES, DEPTH, TO, EPI>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
     if (e != cudaSuccess) return 1000 + (int) e;
     const dim3 grid((M + TILE_M - 1) / TILE_M, (N + TILE_N - 1) / TILE_N);
-    kernel<<<grid, 128, smem, stream>>>(x, w, out, N, M, K);
+    kernel<<<grid, 128, smem, stream>>>(x, w, out, N, M, K, epi);
     return iian_launch_status();
 }
 
-template <int TILE_M, int STAGES, int PER, typename OUT>
-static int launch_rows(const float * x, const float * w, const OUT & out, int N, int M, int K, cudaStream_t stream) {
+template <int TILE_M, int STAGES, int PER, typename TO, typename EPI>
+static int launch_rows(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
     const size_t smem = (size_t) STAGES * (TILE_M + N) * (kRowsK + 4) * sizeof(float);
-    auto kernel = gemm_rows_kernel<TILE_M, STAGES, PER, OUT>;
+    auto kernel = gemm_rows_kernel<TILE_M, STAGES, PER, TO, EPI>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
         if (e != cudaSuccess) return 1000 + (int) e;
     }
-    kernel<<<(M + TILE_M - 1) / TILE_M, kRowsThreads, smem, stream>>>(x, w, out, N, M, K);
+    kernel<<<(M + TILE_M - 1) / TILE_M, kRowsThreads, smem, stream>>>(x, w, out, N, M, K, epi);
     return iian_launch_status();
 }
 
@@ -382,12 +383,12 @@ static int launch_rows(const float * x, const float * w, const OUT & out, int N,
 //   256 x 4,096 x 1,024        70            64               70            82        84
 //   1,024 x 1,024 x 3,072     189           177              189           223       234
 //   2,048 x 6,144 x 4,096   2,023         2,107                                                3,996
-template <typename OUT>
-static int launch_f32(const float * x, const float * w, const OUT & out, int N, int M, int K, cudaStream_t stream) {
+template <typename TO, typename EPI>
+static int launch_f32(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
     if (N <= kRowsMax) {
-        if (M < (N > 8 ? 4096 : 6144)) return launch_rows<8, 6, 1, OUT>(x, w, out, N, M, K, stream);
-        if (N <= 4) return launch_rows<32, 3, 1, OUT>(x, w, out, N, M, K, stream);
-        return N <= 8 ? launch_rows<32, 3, 2, OUT>(x, w, out, N, M, K, stream) : launch_rows<32, 3, 4, OUT>(x, w, out, N, M, K, stream);
+        if (M < (N > 8 ? 4096 : 6144)) return launch_rows<8, 6, 1>(x, w, out, N, M, K, epi, stream);
+        if (N <= 4) return launch_rows<32, 3, 1>(x, w, out, N, M, K, epi, stream);
+        return N <= 8 ? launch_rows<32, 3, 2>(x, w, out, N, M, K, epi, stream) : launch_rows<32, 3, 4>(x, w, out, N, M, K, epi, stream);
     }
     // us per 1,024 of K: `alone` for the first tile of an SM, `more` for each further one that runs beside it (up to `beside`), `then` for
     // those that wait for one of them to end
@@ -399,17 +400,17 @@ static int launch_f32(const float * x, const float * w, const OUT & out, int N, 
     const double wide = cost(64, 128, 65.0, 43.0, 1, 43.0), even = cost(64, 64, 45.0, 13.5, 1, 26.0);
     const double half = cost(32, 64, 24.5, 12.0, 2, 14.8), small = cost(32, 32, 15.0, 7.7, 2, 9.2), least = cost(16, 32, 11.5, 4.1, 2, 5.5);
     const double best = std::min({wide, even, half, small, least});
-    if (wide == best) return launch_tile<64, 128, 8, 8, 1, OUT>(x, w, out, N, M, K, stream);
-    if (even == best) return launch_tile<64, 64, 8, 4, 3, OUT>(x, w, out, N, M, K, stream);
-    if (half == best) return launch_ring<4, 4, 3, 32, OUT>(x, w, out, N, M, K, stream);
-    if (small == best) return launch_ring<4, 2, 4, 64, OUT>(x, w, out, N, M, K, stream);
-    return launch_ring<2, 2, 4, 32, OUT>(x, w, out, N, M, K, stream);
+    if (wide == best) return launch_tile<64, 128, 8, 8, 1>(x, w, out, N, M, K, epi, stream);
+    if (even == best) return launch_tile<64, 64, 8, 4, 3>(x, w, out, N, M, K, epi, stream);
+    if (half == best) return launch_ring<4, 4, 3, 32>(x, w, out, N, M, K, epi, stream);
+    if (small == best) return launch_ring<4, 2, 4, 64>(x, w, out, N, M, K, epi, stream);
+    return launch_ring<2, 2, 4, 32>(x, w, out, N, M, K, epi, stream);
 }
 
-template <typename TX, typename TW, typename OUT>
-static int launch(const void * x, const void * w, const OUT & out, int N, int M, int K, cudaStream_t stream) {
+template <typename TX, typename TW, typename TO, typename EPI>
+static int launch(const void * x, const void * w, void * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
     dim3 grid((M + BM - 1) / BM, (N + BN - 1) / BN);
-    gemm_simt_kernel<TX, TW, OUT><<<grid, 256, 0, stream>>>((const TX *) x, (const TW *) w, out, N, M, K);
+    gemm_simt_kernel<TX, TW, TO, EPI><<<grid, 256, 0, stream>>>((const TX *) x, (const TW *) w, (TO *) out, N, M, K, epi);
     return iian_launch_status();
 }
 
@@ -424,20 +425,18 @@ IIAN_API int iian_gemm_simt(const void * x, int x_dtype, const void * w, int w_d
     if ((M + BM - 1) / BM > 2147483647 || (N + BN - 1) / BN > 65535) return IIAN_ERR_LIMIT;
     typedef __nv_bfloat16 bf;
     if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32 && K % 4 == 0 && ((uintptr_t) x | (uintptr_t) w) % 16 == 0)
-        return out_dtype == IIAN_F32 ? launch_f32((const float *) x, (const float *) w, PlainOut<float>{(float *) out, M}, N, M, K, stream)
-             : out_dtype == IIAN_BF16 ? launch_f32((const float *) x, (const float *) w, PlainOut<bf>{(bf *) out, M}, N, M, K, stream) : (int) IIAN_ERR_DTYPE;
-    const PlainOut<float> f = {(float *) out, M};
-    const PlainOut<bf> h = {(bf *) out, M};
+        return out_dtype == IIAN_F32 ? launch_f32((const float *) x, (const float *) w, (float *) out, N, M, K, Plain(), stream)
+             : out_dtype == IIAN_BF16 ? launch_f32((const float *) x, (const float *) w, (bf *) out, N, M, K, Plain(), stream) : (int) IIAN_ERR_DTYPE;
     const int key = x_dtype * 4 + w_dtype * 2 + out_dtype;
     switch (key) {
-        case 0: return launch<float, float>(x, w, f, N, M, K, stream);
-        case 1: return launch<float, float>(x, w, h, N, M, K, stream);
-        case 2: return launch<float, bf>(x, w, f, N, M, K, stream);
-        case 3: return launch<float, bf>(x, w, h, N, M, K, stream);
-        case 4: return launch<bf, float>(x, w, f, N, M, K, stream);
-        case 5: return launch<bf, float>(x, w, h, N, M, K, stream);
-        case 6: return launch<bf, bf>(x, w, f, N, M, K, stream);
-        case 7: return launch<bf, bf>(x, w, h, N, M, K, stream);
+        case 0: return launch<float, float, float>(x, w, out, N, M, K, Plain(), stream);
+        case 1: return launch<float, float, bf>(x, w, out, N, M, K, Plain(), stream);
+        case 2: return launch<float, bf, float>(x, w, out, N, M, K, Plain(), stream);
+        case 3: return launch<float, bf, bf>(x, w, out, N, M, K, Plain(), stream);
+        case 4: return launch<bf, float, float>(x, w, out, N, M, K, Plain(), stream);
+        case 5: return launch<bf, float, bf>(x, w, out, N, M, K, Plain(), stream);
+        case 6: return launch<bf, bf, float>(x, w, out, N, M, K, Plain(), stream);
+        case 7: return launch<bf, bf, bf>(x, w, out, N, M, K, Plain(), stream);
     }
     return IIAN_ERR_DTYPE;
 }
@@ -448,16 +447,16 @@ IIAN_API int iian_linear_act_simt(const void * x, int x_dtype, long long ldx, co
                                   int K, int act, cudaStream_t stream) {
     if (N <= 0 || M <= 0) return IIAN_OK;
     if (K <= 0 || ldx < K) return IIAN_ERR_SHAPE;
-    if ((N + BN - 1) / BN > 65535) return IIAN_ERR_LIMIT;
+    if ((N + BN - 1) / BN > 65535 || ldx > 2147483647LL) return IIAN_ERR_LIMIT;
     typedef __nv_bfloat16 bf;
-    FusedOut f = {};
+    Fused f = {};
     if (!linear_epilogue(f.e, bias, residual, res_dtype, ldr, out, out_dtype, ldo, act)) return IIAN_ERR_DTYPE;
-    f.ld = ldx;
+    f.ldx = (int) ldx;
     if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32 && K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t) x | (uintptr_t) w) % 16 == 0)
-        return launch_f32((const float *) x, (const float *) w, f, N, M, K, stream);
-    if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32) return launch<float, float>(x, w, f, N, M, K, stream);
-    if (x_dtype == IIAN_F32 && w_dtype == IIAN_BF16) return launch<float, bf>(x, w, f, N, M, K, stream);
-    if (x_dtype == IIAN_BF16 && w_dtype == IIAN_F32) return launch<bf, float>(x, w, f, N, M, K, stream);
-    if (x_dtype == IIAN_BF16 && w_dtype == IIAN_BF16) return launch<bf, bf>(x, w, f, N, M, K, stream);
+        return launch_f32((const float *) x, (const float *) w, (float *) nullptr, N, M, K, f, stream);
+    if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32) return launch<float, float, float>(x, w, nullptr, N, M, K, f, stream);
+    if (x_dtype == IIAN_F32 && w_dtype == IIAN_BF16) return launch<float, bf, float>(x, w, nullptr, N, M, K, f, stream);
+    if (x_dtype == IIAN_BF16 && w_dtype == IIAN_F32) return launch<bf, float, float>(x, w, nullptr, N, M, K, f, stream);
+    if (x_dtype == IIAN_BF16 && w_dtype == IIAN_BF16) return launch<bf, bf, float>(x, w, nullptr, N, M, K, f, stream);
     return IIAN_ERR_DTYPE;
 }
