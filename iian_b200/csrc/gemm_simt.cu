@@ -333,7 +333,10 @@ gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int n = g + i * GROUPS;
-        if (n < N && m0 + m < M) put_out(out, epi, n, m0 + m, M, acc[i]);
+        if (n < N && m0 + m < M) {
+            if constexpr (EPI::fused) epi.e.store(acc[i], (size_t) n, m0 + m);
+            else out[(size_t) n * M + m0 + m] = from_f32<TO>(acc[i]);
+        }
     }
 }
 

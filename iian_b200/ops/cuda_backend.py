@@ -78,14 +78,46 @@ def _stream() -> int:
     return _PINNED_STREAM[0] or torch.cuda.current_stream().cuda_stream
 
 
+_entries = {}
+
+
+def _entry(lib_name: str, fn_name: str, argtypes):
+    """``_fn`` for calls of a few microseconds: the library's entry point is looked up once."""
+    fn = _entries.get(fn_name)
+    if fn is None:
+        fn = _entries[fn_name] = _fn(lib_name, fn_name, argtypes)
+    return fn
+
+
 def _device_stream(*tensors) -> int:
     """The stream to launch on for tensors that all lie on the current device (a kernel of one device cannot be launched on another's
     stream); anything else is refused."""
-    here = torch._C._cuda_getDevice()
+    here = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
-            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+            raise KernelError(f"a tensor is on {t.device}, another on {tensors[0].device}")
+    if here < 0:
+        raise KernelError(f"tensors are on {tensors[0].device}; the engine's kernels run on CUDA only")
+    if here != torch._C._cuda_getDevice():
+        raise KernelError(f"tensors are on cuda:{here}, the current device is cuda:{torch._C._cuda_getDevice()}")
     return _PINNED_STREAM[0] or torch._C._cuda_getCurrentRawStream(here)
+
+
+def _row_place(t: torch.Tensor, what: str):
+    """(pointer, row distance) of a matrix whose rows are contiguous (a column slice of a wider matrix is fine)."""
+    place = t.stride()
+    if len(place) != 2 or (place[1] != 1 and t.shape[1] > 1):
+        raise KernelError(f"{what}: expected a matrix with contiguous rows")
+    return t.data_ptr(), place[0]
+
+
+def _whole(t: Optional[torch.Tensor], what: str, dtype=None) -> int:
+    """Pointer of a contiguous tensor of this type (0 for None); where it lies is ``_device_stream``'s to say."""
+    if t is None:
+        return 0
+    if (dtype is not None and t.dtype != dtype) or not t.is_contiguous():
+        raise KernelError(f"{what}: expected a contiguous tensor" + (f" of {dtype}, got {t.dtype}" if dtype is not None else ""))
+    return t.data_ptr()
 
 
 class pin_stream:
@@ -138,6 +170,20 @@ def _fn(lib_name: str, fn_name: str, argtypes):
         fn.restype = c_int
         _sigs_done.add(key)
     return fn
+
+
+# argument types of the entry points that are called most often for least work, laid out once
+_MOE_ROUTE_GROUPED_ARGS = [c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                           c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p]
+_LINEAR_ACT_ARGS = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int,
+                    c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+_LINEAR_ACT_SIMT_ARGS = [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
+                         c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p]
+_LINEAR_LOGPROBS_TILES_ARGS = [c_int, c_int, c_int]
+_LINEAR_LOGPROBS_ARGS = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                         c_int, c_int, c_float, c_int, c_void_p, c_void_p]
+_LINEAR_LOGPROBS_PIECE_ARGS = [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]
+_LINEAR_LOGPROBS_JOIN_ARGS = [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
 
 
 class CudaKernels:
@@ -2290,21 +2336,23 @@ class CudaKernels:
         ``top`` experts with the largest ``c`` are taken, largest first; ties go to the lower index, and scores are compared in 64 bits.  An
         expert weighs ``scale * s``, with ``renormalise`` divided by the sum of the chosen ``s`` (0 where that is 0).  E up to 1,024, up to
         32 groups and 32 experts a token."""
+        if logits.dim() != 2:
+            raise KernelError("moe_route_grouped: logits float32 [N, E]")
         n, e = logits.shape
         if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top) or (correction is not None and correction.numel() != e):
             raise KernelError("moe_route_grouped: logits float32 [N, E]; correction [E]; ids / weights [N, top]")
-        if score not in ("sigmoid", "softmax"):
+        if score != "sigmoid" and score != "softmax":
             raise KernelError(f"moe_route_grouped: score is 'sigmoid' or 'softmax', not {score!r}")
         if groups < 1 or e % groups or not 1 <= top_groups <= groups or group_top not in (1, 2) or not 1 <= top <= top_groups * (e // groups):
             raise KernelError(f"moe_route_grouped: {top} of {e} experts, {top_groups} of {groups} groups known by their best {group_top}")
-        lp, ld = self._rows(logits, "router logits")
+        lp, ld = _row_place(logits, "router logits")
+        cp, ip = _whole(correction, "choice correction", torch.float32), _whole(ids, "expert ids", torch.int32)
+        wp = _whole(weights, "expert weights", torch.float32)
         stream = _device_stream(logits, ids, weights, correction)
         if n == 0:
             return
-        fn = _fn("moe_groups", "iian_moe_route_grouped", [c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                                          c_float, c_void_p, c_void_p, c_int, c_void_p])
-        _check(fn(lp, ld, _cuda(correction, "choice correction", torch.float32), e, groups, top_groups, group_top, top, int(score == "softmax"),
-                  int(renormalise), scale, _cuda(ids, "expert ids", torch.int32), _cuda(weights, "expert weights", torch.float32), n, stream),
+        fn = _entry("moe_groups", "iian_moe_route_grouped", _MOE_ROUTE_GROUPED_ARGS)
+        _check(fn(lp, ld, cp, e, groups, top_groups, group_top, top, 1 if score == "softmax" else 0, 1 if renormalise else 0, scale, ip, wp, n, stream),
                "moe_route_grouped")
 
     # ---- products with what follows them in their epilogue (csrc/linear_fused.cu, csrc/gemm_simt.cu) ------------------------------
@@ -2312,20 +2360,20 @@ class CudaKernels:
 
     @staticmethod
     def _product_rows(x: torch.Tensor, w: torch.Tensor, what: str):
-        """(pointer of x, row stride, whether the tensor cores' product takes x and w) for x [N, K] and w [M, K]."""
-        if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
-            raise KernelError(f"{what}: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
+        """(N, K, M, pointer of x, its row distance, pointer of w, whether the tensor cores' product takes them) for x [N, K] and w [M, K]."""
+        xs, ws = x.shape, w.shape
+        if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[1]:
+            raise KernelError(f"{what}: x {tuple(xs)} and w {tuple(ws)} do not fit")
         if x.dtype not in _CODE or w.dtype not in _CODE:
             raise KernelError(f"{what}: x and w are float32 or bfloat16")
-        n, k = x.shape
-        xp, ld = CudaKernels._rows(x, f"{what} x")
+        n, k = xs
+        xp, ld = _row_place(x, what)
         if n <= 1:
             ld = k
         if k < 1 or ld < k:
             raise KernelError(f"{what}: rows of x overlap or are empty")
-        tc = (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and k % 8 == 0 and ld % 8 == 0 and xp % 16 == 0
-              and w.data_ptr() % 16 == 0)
-        return xp, ld, tc
+        wp = _whole(w, what)
+        return n, k, ws[0], xp, ld, wp, k % 8 == 0 and ld % 8 == 0 and (xp | wp) % 16 == 0 and x.dtype == w.dtype == torch.bfloat16
 
     def linear_act(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
                    residual: Optional[torch.Tensor] = None, form: int = 0) -> None:
@@ -2335,32 +2383,31 @@ class CudaKernels:
         residual and out may be apart.  ``residual`` may be ``out`` itself (the same tensor, or one of the same place, type and row distance);
         other than that out overlaps none of them.  ``activation``: ``none``, ``silu``, ``gelu_tanh``, ``gelu`` (by erf), ``relu``, ``relu2``.  ``form``: a
         tile of the tensor cores' product other than the one it chooses (csrc/linear_fused.cu)."""
-        xp, ldx, tc = self._product_rows(x, w, "linear_act")
-        (n, k), m = x.shape, w.shape[0]
+        n, k, m, xp, ldx, wp, tc = self._product_rows(x, w, "linear_act")
         act = self.LINEAR_ACTIVATIONS.get(activation)
         if act is None:
             raise KernelError(f"linear_act: activation {activation!r} has no kernel ({', '.join(self.LINEAR_ACTIVATIONS)})")
         if out.shape != (n, m) or (bias is not None and bias.numel() != m) or (residual is not None and residual.shape != (n, m)):
             raise KernelError(f"linear_act: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}, bias [M], residual [N, M] do not fit")
-        oc, op, ldo = _code(out, "linear_act out"), *self._rows(out, "linear_act out")
-        rc, rp, ldr = (_code(residual, "linear_act residual"), *self._rows(residual, "linear_act residual")) if residual is not None else (0, 0, 0)
+        oc, (op, ldo) = _code(out, "linear_act out"), _row_place(out, "linear_act out")
         if n > 1 and ldo < m:
             raise KernelError("linear_act: rows of out overlap")
-        if rp and rp == op and (rc != oc or (n > 1 and ldr != ldo)):
-            raise KernelError("linear_act: a residual in the place of out has its type and row distance")
+        rc = rp = ldr = 0
+        if residual is not None:
+            rc, (rp, ldr) = _code(residual, "linear_act residual"), _row_place(residual, "linear_act residual")
+            if rp == op and (rc != oc or (n > 1 and ldr != ldo)):
+                raise KernelError("linear_act: a residual in the place of out has its type and row distance")
+        bp = _whole(bias, "linear_act bias", torch.float32)
         stream = _device_stream(x, w, out, bias, residual)
         if n == 0 or m == 0:
             return
-        wp, bp = _cuda(w, "linear_act w"), _cuda(bias, "linear_act bias", torch.float32)
         if tc:
             status = self.tcgen05_status_buffer(x.device).data_ptr()
             CudaKernels._tc_used = True
-            fn = _fn("linear_fused", "iian_linear_act", [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int,
-                                                         c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+            fn = _entry("linear_fused", "iian_linear_act", _LINEAR_ACT_ARGS)
             _check(fn(xp, ldx, wp, bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, form, status, stream), "linear_act")
             return
-        fn = _fn("gemm_simt", "iian_linear_act_simt", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
-                                                       c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p])
+        fn = _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
         _check(fn(xp, _CODE[x.dtype], ldx, wp, _CODE[w.dtype], bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, stream), "linear_act_simt")
 
     SCORE_ROWS = 16384          # rows of one launch: their partial sums take up to 8 bytes a row and 128 columns
@@ -2374,29 +2421,27 @@ class CudaKernels:
         x [N, K] (rows may be apart) and w [V, K] float32 or bfloat16, targets int32 [N].  A negative target is none: its log-probability is
         0; one of V or more gives what is no number.  A row of nothing but minus infinity has the log-sum-exp minus infinity.  The working
         memory, a pair of floats a row and some 200 columns, is the call's own."""
-        xp, ldx, tc = self._product_rows(x, w, "linear_logprobs")
-        (n, k), v = x.shape, w.shape[0]
+        n, k, v, xp, ldx, wp, tc = self._product_rows(x, w, "linear_logprobs")
         if targets.shape != (n,) or logprobs.shape != (n,) or lse.shape != (n,) or v < 1:
             raise KernelError(f"linear_logprobs: x {tuple(x.shape)}, w {tuple(w.shape)}; targets, logprobs and lse [N] do not fit")
         cap = float(softcap) if softcap is not None else 0.0
         if not 0.0 <= cap < float("inf") or (softcap is not None and cap == 0.0):
             raise KernelError("linear_logprobs: softcap must be positive")
-        tp, op, sp = (_cuda(targets, "linear_logprobs targets", torch.int32), _cuda(logprobs, "linear_logprobs out", torch.float32),
-                      _cuda(lse, "linear_logprobs lse", torch.float32))
+        tp, op = _whole(targets, "linear_logprobs targets", torch.int32), _whole(logprobs, "linear_logprobs out", torch.float32)
+        sp = _whole(lse, "linear_logprobs lse", torch.float32)
         if op == sp and n > 0:
             raise KernelError("linear_logprobs: logprobs and lse are two tensors")
         stream = _device_stream(x, w, targets, logprobs, lse)
-        wp, esize = _cuda(w, "linear_logprobs w"), x.element_size()
+        esize = x.element_size()
         for r in range(0, n, self.SCORE_ROWS):
             t = min(self.SCORE_ROWS, n - r)
             at = (tp + 4 * r, op + 4 * r, sp + 4 * r)
             if tc:
                 status = self.tcgen05_status_buffer(x.device).data_ptr()
                 CudaKernels._tc_used = True
-                tiles = _fn("linear_fused", "iian_linear_logprobs_tiles", [c_int, c_int, c_int])(t, v, form)
+                tiles = _entry("linear_fused", "iian_linear_logprobs_tiles", _LINEAR_LOGPROBS_TILES_ARGS)(t, v, form)
                 part = torch.empty(2 * max(1, tiles) * t, dtype=torch.float32, device=x.device)
-                fn = _fn("linear_fused", "iian_linear_logprobs", [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                                                  c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+                fn = _entry("linear_fused", "iian_linear_logprobs", _LINEAR_LOGPROBS_ARGS)
                 _check(fn(xp + r * ldx * esize, ldx, wp, *at, part.data_ptr(), t, v, k, cap, form, status, stream), "linear_logprobs")
                 LAUNCHES[0] += 1
                 continue
@@ -2409,16 +2454,14 @@ class CudaKernels:
         pieces = -(-v // width)
         logits = torch.empty(t * width, dtype=torch.float32, device=x.device)
         part = torch.empty(2 * pieces * splits * t, dtype=torch.float32, device=x.device)
-        product = _fn("gemm_simt", "iian_linear_act_simt", [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
-                                                            c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p])
-        take = _fn("linear_fused", "iian_linear_logprobs_piece", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                                                                  c_float, c_void_p])
+        product = _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
+        take = _entry("linear_fused", "iian_linear_logprobs_piece", _LINEAR_LOGPROBS_PIECE_ARGS)
         for i in range(pieces):
             v0, p = i * width, min(width, v - i * width)
             _check(product(xp, _CODE[x.dtype], ldx, wp + v0 * k * w.element_size(), _CODE[w.dtype], 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k,
                            0, stream), "linear_act_simt")
             _check(take(logits.data_ptr(), t, p, v0, at[0], at[1], part.data_ptr(), i * splits, splits, cap, stream), "linear_logprobs_piece")
-        join = _fn("linear_fused", "iian_linear_logprobs_join", [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+        join = _entry("linear_fused", "iian_linear_logprobs_join", _LINEAR_LOGPROBS_JOIN_ARGS)
         _check(join(part.data_ptr(), pieces * splits, t, v, *at, stream), "linear_logprobs_join")
 
     # ---- sampling ------------------------------------------------------------------------
