@@ -10,8 +10,9 @@
 // than these can tell, does its token again in 64.  A score that is no number is the smallest; a row whose chosen scores are all 0
 // weighs 0 (a softmax over logits of minus infinity alone is such a row).
 //
-// What bounds it: the integer pipe, that is the chain of `top` reductions and the groups' ranks.  8,192 tokens, 8 of 256 experts in 8 groups: 14.5 us, 24
-// with all scores in 64 bits; a decode step's 61 tokens 2.8, the launch.
+// What bounds it: the integer pipe, that is the chain of `top` reductions and the groups' ranks, and the latency of the tokens that need 64
+// bits.  Sigmoid scores with a correction, 8 of 256 experts in 8 groups: 61 tokens 3.4 us (2.3 of them the launch), 512 4.1, 2,047 6.2, 8,192 10.8
+// (8.9 MB: 0.8 TB/s); every score in 64 bits 24 us, neighbours left to route_exact 14.5.
 #include "common.cuh"
 
 namespace iian {
@@ -173,11 +174,13 @@ template <int SLOTS> __device__ __forceinline__ void sort_keys(unsigned (&k)[SLO
 // The same in 32 bits.  A sigmoid is off by less than 4e-7 (2 units in the last place each of the exponential and the reciprocal, which
 // matter most at 1, and the rounding of the sum between them), a softmax by less than 5e-6 of the row's largest score (the exponentials'
 // sum, 64 terms in a lane, has most of it), and the corrected score by half a unit of its own more.  Two of them whose order decides
-// anything -- neighbours among the chosen and the first that is not, the last group taken and the first that is not -- and that are nearer
-// than twice that leave the token to route_exact, as do scores that are no finite numbers.
+// anything -- neighbours among the chosen and the first that is not, the last group taken and the first that is not -- may be nearer than twice
+// that.  Outputs and groups are then put in order by their scores in 64 bits, an output or two a lane; more than one output at the border, softmax
+// scores with a correction and scores that are no finite numbers leave the token to route_exact (whose latency, 5 us, was the whole call's as
+// soon as one token in it took that way: 512 tokens 8.3 us, 61 tokens 2.9).
 // Up to 8 outputs a lane, the lowest bits of a key give way to the output's slot (SLOTS units in the last place, which widen that border) and a
 // lane sorts its keys: a choice is then a reduction and a step down the winner's list, a third of the instructions of looking at all of
-// them again (8,192 tokens, 8 of 256: 17.5 us with that, bound by the integer pipe).
+// them again (8,192 tokens, 8 of 256: 17.5 us with that where sorted keys took 14.5); 16 and more outputs a lane are slower sorted (24 against 19).
 template <int SLOTS>
 __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs p, int N, int vec) {
     pdl_launch_dependents();
@@ -231,6 +234,10 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs 
     const float base = p.softmax ? 1e-5f : 2e-6f;
     auto number = [](unsigned k) { return __int_as_float((int) (k & 0x80000000u ? k ^ 0x80000000u : ~k)); };
     auto near_of = [&](float v) { return base * most + (base + (SORT ? SLOTS * 1.2e-7f : 0.0f)) * fabsf(v); };
+    auto exact_score = [&](int e) {                          // of a sigmoid, or of a softmax without a correction as a multiple of the row's sum
+        const double x = p.logits[t * p.ld + e];
+        return p.softmax ? exp(x - (double) mx) : 1.0 / (1.0 + exp(-x)) + (p.correction != nullptr ? (double) p.correction[e] : 0.0);
+    };
     unsigned key[SLOTS];                                     // 0: not to be chosen
 #pragma unroll
     for (int i = 0; i < SLOTS; i++) key[i] = i < held ? (order_key(s[i] + c[i]) & ~SLOT_BITS) | (SLOT_BITS - (SORT ? i : 0)) : 0;
@@ -260,33 +267,65 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs 
             const float other = __shfl_sync(0xffffffffu, gs, g * p.lanes);
             ahead += other > gs || (other == gs && g < group);
         }
-        const bool shut = ahead >= p.top_groups, live = group < p.groups;
+        bool shut = ahead >= p.top_groups;
+        const bool live = group < p.groups;
         const float lo = number(__reduce_min_sync(0xffffffffu, live && !shut ? order_key(gs) : 0xffffffffu));
         const float hi = number(__reduce_max_sync(0xffffffffu, live && shut ? order_key(gs) : 0u));
         // (the two that a group's score is made of may lie further from 0 than it does)
         const float widest = two ? fmaxf(fabsf(number(k1)), fabsf(number(k2))) : fabsf(gs);
-        unsure = live && (!(widest < 1e30f) || !(lo - hi > 2.0f * near_of(widest)));
+        const bool border = live && !(lo - hi > 2.0f * near_of(widest));
+        unsure = live && !(widest < 1e30f);
+        if (__any_sync(0xffffffffu, border)) {
+            // the groups again by the scores in 64 bits of each lane's two largest, where it is certain which these are
+            if constexpr (SORT && SLOTS > 2) {
+                const float third = number(key[2]), second = number(key[1]);
+                unsure = unsure || (held > 2 && !(second - third > near_of(fmaxf(fabsf(second), fabsf(third))))) || (held > 0 && !(fabsf(number(key[0])) < 1e30f));
+            }
+            unsure = unsure || !SORT || (p.softmax && p.correction != nullptr);
+            if (!__any_sync(0xffffffffu, unsure)) {
+                double d1 = -INFINITY, d2 = -INFINITY;
+#pragma unroll 1
+                for (int i = 0; i < min(held, 2); i++) {
+                    const double c64 = exact_score(first + (int) (SLOT_BITS - ((i == 0 ? key[0] : key[SLOTS > 1 ? 1 : 0]) & SLOT_BITS)));
+                    d2 = fmax(d2, fmin(d1, c64));
+                    d1 = fmax(d1, c64);
+                }
+                for (int o = 1; o < p.lanes; o <<= 1) {
+                    const double o1 = shfl_xor_f64(d1, o), o2 = shfl_xor_f64(d2, o);
+                    d2 = fmax(fmax(d2, o2), fmin(d1, o1));
+                    d1 = fmax(d1, o1);
+                }
+                const double g64 = two ? d1 + d2 : d1;
+                ahead = 0;
+                for (int g = 0; g < p.groups; g++) {
+                    const double other = __shfl_sync(0xffffffffu, g64, g * p.lanes);
+                    ahead += other > g64 || (other == g64 && g < group);
+                }
+                shut = ahead >= p.top_groups;
+            }
+        }
         if (shut) {
 #pragma unroll
             for (int i = 0; i < SLOTS; i++) key[i] = 0;
         }
     }
-    // The chain: a lane holds its best key; the warp's best goes to choice k, and the lane that had it leaves its output's number behind.  Equal
-    // keys, in one lane or in two, leave the token to route_exact too.
-    __shared__ int taken[4][kGroupTopMost + 1];
+    // The chain: a lane holds its best key; the warp's best goes to choice k, and the lane that had it -- the first of them -- leaves its output's
+    // number behind.  Two more than are taken: the first that is not, and how near the next one comes to it.
+    __shared__ int taken[4][kGroupTopMost + 2];
     int * chosen = taken[threadIdx.x >> 5];
-    unsigned best = key[0], mine_key = 0, last_key = 0;
+    unsigned best = key[0], mine_key = 0, edge_key = 0, beyond_key = 0;
     if constexpr (!SORT) {
 #pragma unroll
         for (int i = 0; i < SLOTS; i++) best = max(best, key[i]);
     }
-    for (int k = 0; k <= p.top; k++) {                       // (one more than are taken: how near it comes)
+    for (int k = 0; k < p.top + 2; k++) {
         const unsigned won = __reduce_max_sync(0xffffffffu, best);
         if (lane == k) mine_key = won;
-        last_key = won;                                      // (0: every output that there was is taken)
+        if (k == p.top) edge_key = won;
+        if (k == p.top + 1) beyond_key = won;
+        if (won == 0) break;                                 // every output that there was is taken
         const unsigned who = __ballot_sync(0xffffffffu, best == won);
-        unsure = unsure || ((who & (who - 1)) != 0 && won != 0);
-        if (best == won) {
+        if (lane == __ffs(who) - 1) {
             if constexpr (SORT) {
                 chosen[k] = first + (int) (SLOT_BITS - (won & SLOT_BITS));
 #pragma unroll
@@ -294,26 +333,47 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs 
                 key[SLOTS - 1] = 0;
                 best = key[0];
             } else {
-                int at = 0, equal = 0;
+                int at = 0;
+                bool found = false;
                 best = 0;
 #pragma unroll
                 for (int i = 0; i < SLOTS; i++) {
-                    if (key[i] == won) { key[i] = 0; at = i; equal++; }
+                    if (key[i] == won && !found) { key[i] = 0; at = i; found = true; }
                     best = max(best, key[i]);
                 }
                 chosen[k] = first + at;
-                unsure = unsure || (equal > 1 && won != 0);
             }
         }
     }
     __syncwarp();
-    const float v = number(mine_key), before = __shfl_up_sync(0xffffffffu, v, 1), after = number(last_key);
-    if (lane < p.top) {
-        unsure = unsure || !(fabsf(v) < 1e30f) || (lane > 0 && !(before - v > near_of(fmaxf(fabsf(before), fabsf(v)))))
-              || (lane == p.top - 1 && last_key != 0 && !(v - after > near_of(fmaxf(fabsf(after), fabsf(v)))));
+    // which places are nearer to the one before than 32 bits can tell
+    const float v = number(mine_key), before = __shfl_up_sync(0xffffffffu, v, 1);
+    const bool there = lane <= p.top && mine_key != 0;
+    const bool close = there && lane > 0 && v > -1e30f && !(before - v > near_of(fmaxf(fabsf(before), fabsf(v))));
+    unsure = unsure || (lane < p.top && !(fabsf(v) < 1e30f));
+    unsigned tied = __ballot_sync(0xffffffffu, close && lane < p.top);
+    const float last = __shfl_sync(0xffffffffu, v, p.top - 1), edge = number(edge_key), beyond = number(beyond_key);
+    if (edge_key != 0 && edge > -1e30f && !(last - edge > near_of(fmaxf(fabsf(last), fabsf(edge))))) {
+        tied |= 1u;                                          // the first that is not may have to be; it cannot be told from more of them, nor has it
+        unsure = unsure || p.top == 32 ||                    // a lane behind 32 choices
+                 (beyond_key != 0 && beyond > -1e30f && !(edge - beyond > near_of(fmaxf(fabsf(edge), fabsf(beyond)))));
     }
+    if (p.softmax && p.correction != nullptr && tied != 0) unsure = true;         // (would need the row's sum in 64 bits)
     unsure = __any_sync(0xffffffffu, unsure);
-    const int mine_e = lane < p.top && !unsure ? chosen[lane] : 0;
+    int mine_e = there && !unsure ? chosen[lane] : 0;
+    if (tied != 0 && !unsure) {
+        // those that were chosen and the first that was not, put in the order that they have in 64 bits
+        const double c64 = there ? exact_score(mine_e) : -INFINITY;
+        int place = 0;
+        for (int j = 0; j < min(p.top + 1, 32); j++) {
+            const double other = __shfl_sync(0xffffffffu, c64, j);
+            const int e = __shfl_sync(0xffffffffu, mine_e, j);
+            place += other > c64 || (other == c64 && e < mine_e);
+        }
+        if (there) chosen[place] = mine_e;
+        __syncwarp();
+        mine_e = chosen[lane < p.top ? lane : 0];
+    }
     float mine = 0.0f;
     if (lane < p.top) {
         const float x = p.logits[t * p.ld + mine_e];
