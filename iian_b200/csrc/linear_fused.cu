@@ -8,15 +8,21 @@
 // up to 256).  Warp 0 brings both operands by TMA, K in blocks of 64, warp 1 multiplies, warps 2..5 run the epilogue on a thread's own
 // row of the accumulator while the next tile is multiplied into the other one.
 //
-// Few rows of x: a stage holds only the rows there are (in eights), so that nearly all of shared memory is weights on their way.  The
-// product then still reads 128 rows of shared memory; what lies behind the real ones only reaches rows of the accumulator that nobody
-// reads.
+// Few rows of x: the rows of w are the product's and those of x its columns (SWAP), up to 128 of w a tile and all of x, in sixteens.  The
+// accumulator then has a row of w in a lane: the epilogue turns it around in shared memory, the softmax's sums are taken over the lanes.
+// Where x's rows stay the product's although there are fewer than 128, a stage holds only those there are (in eights).  In either case a tile
+// may have fewer rows than the 128 that the product reads of shared memory; what lies behind the real ones only reaches rows of the
+// accumulator that nobody reads.
 //
 // Few tiles: the K blocks of a tile are shared by a cluster of `ks` CTAs.  Each leaves its part in its shared memory, and each adds up all
 // parts, in their order, for its share of the tile.
 //
 // The softmax's sums: a thread walks its row's columns with a running maximum and sum and leaves them per tile; a second kernel joins a
 // row's.  The maximum is the running one, so no exponential overflows; an empty sum has the maximum minus infinity.
+//
+// Launches are programmatic (common.cuh): set-up runs beside the end of the kernel before (1 x 4,096 x 1,024 8.2 -> 5.7 us).  None announces its
+// own successor early: the joins of scores that were then let in while the product ran cost it 40 to 60 us of 200 (16 and 61 rows), and
+// products gain nothing by it.
 //
 // Every wait is bounded, as in gemm_tcgen05.cu; a producer that gives up waits, bounded too, for the copies it still has under way.
 #include <math_constants.h>
@@ -52,7 +58,7 @@ struct LfScore {
 enum { LF_SCORE = 0, LF_ANY = 1, LF_BF16 = 2, LF_F32 = 3, LF_BF16_RES = 4, LF_F32_RES = 5 };       // (the residual of the last two is float32)
 
 struct LfArgs {
-    int T, N, bn, ks, stages, stage_bytes, a_bytes, kb_bytes, all_kb, m_tiles, num_tiles, units;
+    int T, N, bn, ks, x_cols, stages, stage_bytes, a_bytes, kb_bytes, all_kb, m_tiles, num_tiles, units;
     // where K is shared: a CTA adds up `per` of the tile's groups of 4 columns (inv_per = 65536 / per, rounded up); the parts arrive at
     // recv_off, rows of recv_ld groups for every CTA that sends, over the ring (recv_shared) or behind it
     int per, inv_per, recv_off, recv_ld, recv_rows, recv_shared;
@@ -99,6 +105,29 @@ __device__ __forceinline__ void lf_sum(unsigned taddr, int accs, int between, fl
 #pragma unroll
         for (int i = 0; i < LF_COLS; i++) y[i] += __uint_as_float(r[i]);
     }
+}
+
+// LF_COLS columns of 32 lanes turned around: `turn` holds a column's 32 lanes side by side afterwards.  A whole warp calls it.
+__device__ __forceinline__ void lf_turn(unsigned taddr, int accs, int between, float * turn, int lane) {
+    float r[LF_COLS];
+    lf_sum(taddr, accs, between, r);
+    __syncwarp();                                            // the columns before have been read
+#pragma unroll
+    for (int j = 0; j < LF_COLS; j++) turn[j * 32 + lane] = r[j];
+    __syncwarp();
+}
+
+// One value of 32 columns in every lane becomes, in lane c, column c's value over all lanes.
+template <typename OP> __device__ __forceinline__ float lf_over_lanes(float (&v)[32], int lane, OP op) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; i++) {
+            const bool up = lane & o;
+            const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+        }
+    return v[0];
 }
 
 // 32 columns of a row, `live` of them in the matrix, into the row's running maximum and sum
@@ -149,7 +178,7 @@ template <int KIND> __device__ __forceinline__ void lf_put(const LinearEpilogue 
     }
 }
 
-template <bool PAIR, int KIND>
+template <bool PAIR, bool SWAP, int KIND>
 __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b, const LfArgs p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -168,28 +197,27 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
     const int block = PAIR ? (int) blockIdx.x >> 1 : (int) blockIdx.x, unit = p.ks > 1 ? block / p.ks : block;
     const int a_bytes = p.a_bytes, kb_bytes = p.kb_bytes;
     const int kb0 = p.ks > 1 ? p.all_kb * split / p.ks : 0, kb1 = p.ks > 1 ? p.all_kb * (split + 1) / p.ks : p.all_kb;
-    const int acc_cols = (bn + 31) & ~31;
+    const int acc_cols = ((SWAP ? p.x_cols : bn) + 31) & ~31;
     const int early = PAIR || unit >= num_tiles ? 0 : min(stages, kb1 - kb0);  // copies that are asked for before anything else is set up
 
-    auto copy = [&](int s, int kb, int m0, int n0) {
+    auto copy = [&](int s, int kb, int ya, int yb) {
         const unsigned to = smem_addr(smem + s * p.stage_bytes);
         if constexpr (PAIR) {
             const unsigned bar = map_to_cta(smem_addr(&full_bar[s]), leader);
             if (rank == 0) mbar_expect_tx_warp(smem_addr(&full_bar[s]), 2 * KPS * kb_bytes);
 #pragma unroll
             for (int j = 0; j < KPS; j++) {
-                tma_load_2d_pair_warp(to + j * kb_bytes, &map_a, (kb * KPS + j) * TC_BK, m0, bar);
-                tma_load_2d_pair_warp(to + j * kb_bytes + a_bytes, &map_b, (kb * KPS + j) * TC_BK, n0, bar);
+                tma_load_2d_pair_warp(to + j * kb_bytes, &map_a, (kb * KPS + j) * TC_BK, ya, bar);
+                tma_load_2d_pair_warp(to + j * kb_bytes + a_bytes, &map_b, (kb * KPS + j) * TC_BK, yb, bar);
             }
         } else {
             const unsigned bar = smem_addr(&full_bar[s]);
-            mbar_expect_tx_warp(bar, kb_bytes);
-            tma_load_2d_warp(to, &map_a, kb * TC_BK, m0, bar);
-            tma_load_2d_warp(to + a_bytes, &map_b, kb * TC_BK, n0, bar);
+            mbar_expect_tx_warp(bar, SWAP ? (p.bn + p.x_cols) * TC_BK * 2 : kb_bytes);
+            tma_load_2d_warp(to, &map_a, kb * TC_BK, ya, bar);
+            tma_load_2d_warp(to + a_bytes, &map_b, kb * TC_BK, yb, bar);
         }
     };
 
-    pdl_launch_dependents();
     if (warp == 0) {
         if (lane == 0) {
             for (int s = 0; s < stages; s++) { mbar_init(smem_addr(&full_bar[s]), 1); mbar_init(smem_addr(&empty_bar[s]), 1); }
@@ -198,7 +226,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
         }
         __syncwarp();
         pdl_wait();
-        for (int i = 0; i < early; i++) copy(i, kb0 + i, unit % m_tiles * ROWS, unit / m_tiles * bn);
+        for (int i = 0; i < early; i++) copy(i, kb0 + i, SWAP ? unit * bn : unit % m_tiles * ROWS, SWAP ? 0 : unit / m_tiles * bn);
     }
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -222,11 +250,11 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
         unsigned turn = 0;
         bool gave_up = false;
         for (int tile = unit; tile < num_tiles && !gave_up; tile += units) {
-            const int m0 = tile % m_tiles * ROWS + (int) rank * TC_BM, n0 = tile / m_tiles * bn + (int) rank * half;
+            const int ya = SWAP ? tile * bn : tile % m_tiles * ROWS + (int) rank * TC_BM, yb = SWAP ? 0 : tile / m_tiles * bn + (int) rank * half;
             for (int kb = kb0; kb < kb1; kb++, it++) {
                 if (it >= early) {
                     if (!mbar_wait(smem_addr(&empty_bar[s]), (turn & 1) ^ 1)) { if (lane == 0) { p.status->code = 1; p.status->where = it; } gave_up = true; break; }
-                    copy(s, kb, m0, n0);
+                    copy(s, kb, ya, yb);
                 }
                 if (++s == stages) { s = 0; turn++; }
             }
@@ -242,7 +270,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
         }
     } else if (warp == 1 && rank == 0) {
         // ---- MMA issuer -------------------------------------------------------------------------------------
-        const unsigned idesc = instr_desc_bf16(ROWS, bn);
+        const unsigned idesc = instr_desc_bf16(ROWS, SWAP ? p.x_cols : bn);
         const unsigned long long first = smem_desc_sw128(smem_addr(smem)), to_b = (unsigned long long) (a_bytes >> 4);
         const unsigned long long next_block = (unsigned long long) (kb_bytes >> 4), next_stage = (unsigned long long) (p.stage_bytes >> 4);
         unsigned long long at = first;            // (a ring of 208 KB: the descriptor's 14 bits of address do not overflow)
@@ -298,6 +326,74 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
             }
             tc_fence_after();
             const unsigned acc = tmem_base + ((unsigned) (q * 32) << 16) + (unsigned) (buf * p.buf_cols);
+            if constexpr (SWAP) {
+                // a lane is a row of w, a column one of x
+                const int limit = min(bn, p.N - n0) - q * 32;             // rows of w that this warp's lanes are
+                if constexpr (SCORE) {
+                    // a column's maximum and sum over the lanes: halves of the columns are handed from lane to lane until lane c has column c
+#pragma unroll 1
+                    for (int c0 = half_w * 32; c0 < p.T; c0 += 64) {
+                        unsigned r[32];
+                        tc_ld32(acc + (unsigned) c0, r);
+                        tc_wait_ld();
+                        if (p.accs == 2) {
+                            unsigned r2[32];
+                            tc_ld32(acc + (unsigned) (acc_cols + c0), r2);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
+                        }
+                        float z[32], v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            z[i] = __uint_as_float(r[i]);
+                            if (p.score.cap != 0.0f) z[i] = lf_cap_fast(z[i], p.score.cap, cap_factor);
+                            if (lane >= limit) z[i] = -CUDART_INF_F;
+                            v[i] = z[i];
+                        }
+                        const float m = lf_over_lanes(v, lane, [](float a, float b) { return fmaxf(a, b); });
+                        const float ref = lf_finite_or_zero(m) * kLog2e;
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = lf_exp2(fmaf(z[i], kLog2e, -__shfl_sync(0xffffffffu, ref, i)));
+                        const float s = lf_over_lanes(v, lane, [](float a, float b) { return a + b; });
+                        const int token = c0 + lane, wanted = token < p.T ? p.score.targets[token] : -1, rel = wanted < 0 ? -1 : wanted - n0 - q * 32;
+                        if (token < p.T) p.score.part[((size_t) n_tile * 4 + q) * p.T + token] = make_float2(m, s);
+                        unsigned here = __ballot_sync(0xffffffffu, rel >= 0 && rel < min(limit, 32));
+                        while (here != 0) {                               // (a target among this warp's rows of w)
+                            const int c = __ffs(here) - 1, from = __shfl_sync(0xffffffffu, rel, c);
+                            const float x = __uint_as_float(lf_pick(r, c));
+                            if (lane == from) p.score.lp[c0 + c] = p.score.cap != 0.0f ? p.score.cap * tanhf(x / p.score.cap) : x;
+                            here &= here - 1;
+                        }
+                    }
+                } else if (p.ks == 1 && limit > 0) {
+                    float * turn = reinterpret_cast<float *>(smem + kLfRing) + (warp - 2) * 32 * LF_COLS;
+                    const int in_row = lane / 8, in_col = lane % 8 * 4, col = n0 + q * 32 + in_col, live = limit - in_col;
+                    const float4 bias = lf_bias<KIND>(p.epi, col, live);
+#pragma unroll 1
+                    for (int c0 = half_w * LF_COLS; c0 < p.T; c0 += 2 * LF_COLS) {
+                        float4 res[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int token = c0 + in_row + 4 * i;
+                            res[i] = lf_residual<KIND>(p.epi, (size_t) token, col, token < p.T ? live : 0);
+                        }
+                        lf_turn(acc + (unsigned) c0, p.accs, acc_cols, turn, lane);
+                        float y[16];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float4 v = *reinterpret_cast<const float4 *>(turn + (in_row + 4 * i) * 32 + in_col);
+                            y[4 * i] = v.x + bias.x; y[4 * i + 1] = v.y + bias.y; y[4 * i + 2] = v.z + bias.z; y[4 * i + 3] = v.w + bias.w;
+                        }
+                        linear_act_values<16>(y, p.epi.act);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int token = c0 + in_row + 4 * i;
+                            lf_put<KIND>(p.epi, y + 4 * i, res[i], (size_t) token, col, token < p.T ? live : 0);
+                        }
+                    }
+                }
+            } else
             if (m0 + q * 32 < p.T) {              // (a warp whose rows are all behind the last one has nothing to do)
                 if constexpr (SCORE) {
                     float m = -CUDART_INF_F, s = 0.0f;
@@ -387,7 +483,25 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
                 tc_fence_after();
                 const int q = warp & 3, row = q * 32 + lane;
                 const unsigned acc = tmem_base + ((unsigned) (q * 32) << 16), mine = recv + (unsigned) ((split * p.recv_rows + row) * p.recv_ld) * 16u;
-                if (q * 32 < rows) {
+                if constexpr (SWAP) {
+                    float * turn = reinterpret_cast<float *>(smem + kLfRing) + (warp - 2) * 32 * LF_COLS;
+                    const int in_row = lane / 8, i = q * 8 + lane % 8, owner = (i * p.inv_per) >> 16;
+                    if (q * 32 < bn) {
+#pragma unroll 1
+                        for (int c0 = (warp - 2) / 4 * LF_COLS; c0 < rows; c0 += 2 * LF_COLS) {
+                            lf_turn(acc + (unsigned) c0, p.accs, acc_cols, turn, lane);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const int token = c0 + in_row + 4 * j;
+                                if (token < rows && 4 * i < bn) {
+                                    const float4 v = *reinterpret_cast<const float4 *>(turn + (in_row + 4 * j) * 32 + lane % 8 * 4);
+                                    const unsigned to = map_to_cta(recv + (unsigned) ((split * p.recv_rows + token) * p.recv_ld + i - owner * p.per) * 16u, (unsigned) owner);
+                                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+                                }
+                            }
+                        }
+                    }
+                } else if (q * 32 < rows) {
 #pragma unroll 1
                     for (int c0 = (warp - 2) / 4 * LF_COLS; c0 < bn; c0 += LF_WARPS / 4 * LF_COLS) {
                         float r[LF_COLS];
@@ -439,7 +553,6 @@ constexpr int JOIN_ROWS = 4;
 __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __restrict__ part, int n_tiles, int T, int V,
                                                             const int * __restrict__ targets, float * __restrict__ lp, float * __restrict__ lse) {
     __shared__ float sm[512], ss[512];
-    pdl_launch_dependents();
     pdl_wait();
     constexpr int segs = 512 / JOIN_ROWS, rows = JOIN_ROWS;
     const int r = threadIdx.x % rows, seg = threadIdx.x / rows;
@@ -483,7 +596,6 @@ __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __res
 __global__ void __launch_bounds__(256) logprobs_piece_kernel(const float * __restrict__ logits, int T, int P, int v0, const int * __restrict__ targets,
                                                              float * __restrict__ lp, float2 * __restrict__ part, int first, float cap) {
     __shared__ float sm[8], ss[8];
-    pdl_launch_dependents();
     pdl_wait();
     const size_t row = blockIdx.x;
     const int splits = gridDim.y, c0 = (int) ((long long) P * blockIdx.y / splits), c1 = (int) ((long long) P * (blockIdx.y + 1) / splits);
@@ -534,13 +646,15 @@ static int lf_sms() {
 }
 
 // T, N, bn, ks, status, epi or score as given; PAIR: tiles of 256 rows on pairs of SMs.
-template <bool PAIR, int KIND>
+template <bool PAIR, bool SWAP, int KIND>
 static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, int K, int sms, cudaStream_t stream) {
     constexpr int KPS = PAIR ? 2 : 1, ROWS = PAIR ? 2 * TC_BM : TC_BM;
     // All of it whatever the call needs: two CTAs of a cluster that each waited for the tensor memory of an SM's other CTA, those two in turn
     // waiting for their clusters, would never end, so no SM may hold two.
     constexpr int kRing = kLfRing, smem = kLfSmem, kRecvMost = 80 * 1024;
-    const int a_rows = PAIR || p.T >= TC_BM ? TC_BM : (p.T + 7) / 8 * 8, half = PAIR ? p.bn / 2 : p.bn;
+    if (SWAP && (p.T > TC_BM || p.bn > TC_BM)) return IIAN_ERR_SHAPE;
+    p.x_cols = (p.T + 15) / 16 * 16;                                   // (SWAP: columns of the product; the rows behind the last are zeros)
+    const int a_rows = SWAP ? (p.bn + 7) / 8 * 8 : PAIR || p.T >= TC_BM ? TC_BM : (p.T + 7) / 8 * 8, half = SWAP ? p.x_cols : PAIR ? p.bn / 2 : p.bn;
     p.a_bytes = a_rows * TC_BK * 2;
     p.kb_bytes = p.a_bytes + half * TC_BK * 2;
     p.stage_bytes = KPS * p.kb_bytes;
@@ -550,8 +664,8 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
         p.per = (p.bn / 4 + p.ks - 1) / p.ks;
         p.inv_per = (65536 + p.per - 1) / p.per;
         p.recv_ld = p.per | 1;                                         // an odd number of 16-byte groups: rows of eight lanes meet no bank twice
-        p.recv_rows = a_rows;
-        const int recv = p.ks * a_rows * p.recv_ld * 16;
+        p.recv_rows = SWAP ? p.x_cols : a_rows;
+        const int recv = p.ks * p.recv_rows * p.recv_ld * 16;
         if (recv > kRing) return IIAN_ERR_SHAPE;
         p.recv_shared = recv > kRecvMost;
         if (!p.recv_shared) ring = (kRing - recv) / 1024 * 1024;
@@ -559,19 +673,19 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
     }
     p.stages = std::min(LF_STAGES, (ring - over) / p.stage_bytes);
     p.all_kb = ((K + TC_BK - 1) / TC_BK + KPS - 1) / KPS;
-    p.m_tiles = (p.T + ROWS - 1) / ROWS;
+    p.m_tiles = SWAP ? 1 : (p.T + ROWS - 1) / ROWS;
     const long long tiles = (long long) p.m_tiles * ((p.N + p.bn - 1) / p.bn);
     const int group = (PAIR ? 2 : 1) * p.ks;
     if (tiles * group > 2147483647LL - 65536) return IIAN_ERR_LIMIT;
     p.num_tiles = (int) tiles;
     p.units = p.ks > 1 ? p.num_tiles : std::min(p.num_tiles, sms / group);
-    const int acc_cols = (p.bn + 31) & ~31, bufs = p.units < p.num_tiles ? 2 : 1;      // (a CTA with one tile needs no second buffer)
+    const int acc_cols = ((SWAP ? p.x_cols : p.bn) + 31) & ~31, bufs = p.units < p.num_tiles ? 2 : 1;      // (a CTA with one tile needs no second buffer)
     p.accs = 1;
     while (p.accs < (KIND == LF_SCORE ? 2 : 4) && 2 * p.accs * bufs * acc_cols <= 512 && 2 * p.accs <= p.all_kb / p.ks) p.accs *= 2;
     p.buf_cols = p.accs * acc_cols;
     p.tmem_cols = 32;
     while (p.tmem_cols < (unsigned) (bufs * p.buf_cols)) p.tmem_cols *= 2;
-    auto kernel = linear_fused_kernel<PAIR, KIND>;
+    auto kernel = linear_fused_kernel<PAIR, SWAP, KIND>;
     static bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -581,9 +695,9 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
     }
     if (e != cudaSuccess) return 1000 + (int) e;
     CUtensorMap ma, mb;
-    int rc = make_map(&ma, x, p.T, K, a_rows, ldx);
+    int rc = SWAP ? make_map(&ma, w, p.N, K, p.bn) : make_map(&ma, x, p.T, K, a_rows, ldx);
     if (rc != IIAN_OK) return rc;
-    rc = make_map(&mb, w, p.N, K, half);
+    rc = SWAP ? make_map(&mb, x, p.T, K, p.x_cols, ldx) : make_map(&mb, w, p.N, K, half);
     if (rc != IIAN_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (p.units * group));
@@ -617,39 +731,49 @@ static int lf_check(int T, int N, int K, const void * x, long long ldx, const vo
 
 static int lf_even(int n, int parts, int step) { return std::max(32, ((n + parts - 1) / parts + step - 1) / step * step); }
 
-// The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants are fitted to 26 shapes from
-// 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024, each timed in every form (the form it takes is 2 % slower than the best one on average, 11 % at
-// most).  A K block costs the longest of its copies (128 GB/s an SM, 17 TB/s together), its products, and 0.26 us that a block's
-// instructions and commit take; the operands come from memory at 4.9 TB/s; then come the epilogue of a tile and, where K is shared, the exchange of
-// the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
-static double lf_estimate(int T, int N, int K, int sms, bool pair, int bn, int ks) {
-    const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8;
-    const double tiles = (double) ((T + rows - 1) / rows) * ((N + bn - 1) / bn), ctas = tiles * ks * group;
+// The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants are fitted to 35 shapes from
+// 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024, each timed in every form (the form it takes is 2 % slower than the best one on average, 16 % at
+// most).  A K block costs the longest of its copies (of an SM, and of all together), its products, and the quarter of a microsecond that a
+// block's instructions and commit take; the operands come from memory; then come the epilogue of a tile and, where K is shared, the exchange
+// of the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
+static double lf_estimate(int T, int N, int K, int sms, bool pair, bool swap, int bn, int ks) {
+    const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8, x_cols = (T + 15) / 16 * 16;
+    const double tiles = (swap ? 1.0 : (double) ((T + rows - 1) / rows)) * ((N + bn - 1) / bn), ctas = tiles * ks * group;
     int slots = sms / (group * ks) * (group * ks);
     if (ks > 4) slots = std::min(slots, sms - sms / 9);          // clusters of six or eight leave some SMs of a GPC over
     const double waves = (double) (long long) ((ctas + slots - 1) / slots), active = std::min(ctas, (double) slots);
-    const int kb = ((K + TC_BK - 1) / TC_BK + ks - 1) / ks;
-    const double fill = (a_rows + (pair ? bn / 2 : bn)) * 128.0 / std::min(128e3, 17.1e6 / active), mma = std::max(0.263, bn * 2 / 1850.0 * 1.54);
-    double t = std::max(waves * kb * std::max(fill, mma), 2.0 * K * ((double) N + T) / 4.89e6);
-    if (ks == 1) t += 3.15 * bn / 256 * (a_rows / 128.0 * 0.225 + 0.775);
-    else t += 1.44 + waves * 11.1 * ks * a_rows * (((bn / 4 + ks - 1) / ks) | 1) * 16 / 131072.0;
-    return t;
+    const int kb = ((K + TC_BK - 1) / TC_BK + ks - 1) / ks, per = ((bn / 4 + ks - 1) / ks) | 1;
+    if (swap) {
+        const double block = std::max((bn + x_cols) * 128.0 * active / 12.2e6, std::max(0.217, x_cols * 2 / 1850.0 * 1.96));
+        const double t = std::max(waves * kb * block, 2.0 * K * ((double) N + T) / 5.28e6);
+        return t + (ks == 1 ? 0.17 + 0.86 * T / 128.0 : 1.31 + waves * 6.59 * ks * x_cols * per * 16 / 131072.0);
+    }
+    const double fill = (a_rows + (pair ? bn / 2 : bn)) * 128.0 / std::min(131.5e3, 17.8e6 / active);
+    const double t = std::max(waves * kb * std::max(fill, std::max(0.253, bn * 2 / 1850.0 * 1.5)), 2.0 * K * ((double) N + T) / 3.32e6);
+    return t + (ks == 1 ? 2.74 * bn / 256 : 1.48 + waves * 10.4 * ks * a_rows * per * 16 / 131072.0);
 }
-static void lf_plan(int T, int N, int K, int sms, bool out_f32, bool * pair, int * bn, int * ks) {
+
+// Whether w's rows are the product's: up to 64 rows of x always (1 x 4,096 x 4,096 8.6 us, the other way 10.1; 61 x 4,096 x 12,288 21.6 and 23.5; a
+// row of x then costs 16 columns of a product where it cost 128 rows, and with them the power that bounds a long run of such calls), up to 128
+// where K is long enough to matter (128 x 4,096 x 4,096 13.7 and 14.5, but 100 x 4,096 x 1,024 7.3 and 6.3).
+static bool lf_swaps(int T, int K) { return T <= 64 || (T <= TC_BM && K >= 2048); }
+
+static void lf_plan(int T, int N, int K, int sms, bool out_f32, bool * pair, bool * swap, int * bn, int * ks) {
     struct Known { int T, N, K, sms, f32, pair, bn, ks; };
     static thread_local Known known[16] = {};                // by sizes alone: a model's few products come again and again
     Known & k = known[((unsigned) T * 31u + (unsigned) N * 7u + (unsigned) K) % 16u];
+    *swap = lf_swaps(T, K);
     if (!(k.T == T && k.N == N && k.K == K && k.sms == sms && k.f32 == (int) out_f32 && k.bn > 0)) {
         static const int columns[] = {32, 48, 64, 96, 112, 128, 160, 192, 224, 256}, shares[] = {1, 2, 3, 4, 6};
-        const int blocks = (K + TC_BK - 1) / TC_BK, most = out_f32 && K > 6144 ? 128 : 256;
+        const int blocks = (K + TC_BK - 1) / TC_BK, most = *swap || (out_f32 && K > 6144) ? 128 : 256;
         double best = 1e300;
         for (int p = 0; p < (T > TC_BM ? 2 : 1); p++)
             for (int c : columns)
                 for (int s : shares) {
                     if (c > most || (p && c % 32 != 0) || s > (p ? 4 : 6) || s > (p ? (blocks + 1) / 2 : blocks)) continue;
-                    const long long ctas = (long long) ((T + (p ? 255 : 127)) / (p ? 256 : 128)) * ((N + c - 1) / c) * (p ? 2 : 1);
+                    const long long ctas = (*swap ? 1LL : (long long) ((T + (p ? 255 : 127)) / (p ? 256 : 128))) * ((N + c - 1) / c) * (p ? 2 : 1);
                     if (s > 1 && ctas >= sms) break;
-                    const double t = lf_estimate(T, N, K, sms, p != 0, c, s);
+                    const double t = lf_estimate(T, N, K, sms, p != 0, *swap, c, s);
                     if (t < best) { best = t; k = {T, N, K, sms, (int) out_f32, p, c, s}; }
                     if (c > N) break;
                 }
@@ -664,7 +788,7 @@ static void lf_plan(int T, int N, int K, int sms, bool out_f32, bool * pair, int
 using namespace iian;
 
 // x [T, K] bf16, rows ldx apart; w [N, K] bf16; status: two ints the host reads, as for iian_gemm_tcgen05.  form 0: chosen here; else
-// pair | bn << 1 | ks << 16 (a multiple of 16 from 32 to 256, on pairs of 32; 1 to 8 CTAs that share K, or 1 to 4 pairs).
+// pair | bn << 1 | rows << 14 | ks << 16 (rows: w's rows are the product's, bn up to 128, for x of up to 128 rows; bn a multiple of 16 from 32 to 256, on pairs of 32; 1 to 8 CTAs that share K, or 1 to 4 pairs).
 IIAN_API int iian_linear_act(const void * x, long long ldx, const void * w, const float * bias, const void * residual, int res_dtype,
                              long long ldr, void * out, int out_dtype, long long ldo, int T, int N, int K, int act, int form, int * status,
                              cudaStream_t stream) {
@@ -677,43 +801,48 @@ IIAN_API int iian_linear_act(const void * x, long long ldx, const void * w, cons
     p.T = T; p.N = N;
     p.status = (TcStatus *) status;
     const int blocks = (K + TC_BK - 1) / TC_BK;
-    bool pair = false;
-    if (form == 0) lf_plan(T, N, K, sms, out_dtype == IIAN_F32, &pair, &p.bn, &p.ks);
+    bool pair = false, swap = false;
+    if (form == 0) lf_plan(T, N, K, sms, out_dtype == IIAN_F32, &pair, &swap, &p.bn, &p.ks);
     if (form != 0) {
         pair = form & 1;
-        p.bn = (form >> 1) & 0x7fff;
+        swap = form >> 14 & 1;
+        p.bn = (form >> 1) & 0x1fff;
         p.ks = form >> 16;
-        if (p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0 || p.ks < 1 || p.ks > (pair ? 4 : 8) || p.ks > (pair ? (blocks + 1) / 2 : blocks) || (p.ks > 1 && p.bn / 4 < p.ks)) return IIAN_ERR_SHAPE;
+        if ((swap && (pair || T > TC_BM || p.bn > TC_BM)) || p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0 || p.ks < 1 || p.ks > (pair ? 4 : 8) || p.ks > (pair ? (blocks + 1) / 2 : blocks) || (p.ks > 1 && p.bn / 4 < p.ks)) return IIAN_ERR_SHAPE;
     }
     const LinearEpilogue & e = p.epi;
     const bool whole = N % 4 == 0 && e.out_vec && (bias == nullptr || e.bias_vec) && (residual == nullptr || (e.res_vec && !e.res_bf16));
     auto go = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;
-        return pair ? lf_launch<true, KIND>(p, x, ldx, w, K, sms, stream) : lf_launch<false, KIND>(p, x, ldx, w, K, sms, stream);
+        return pair ? lf_launch<true, false, KIND>(p, x, ldx, w, K, sms, stream)
+             : swap ? lf_launch<false, true, KIND>(p, x, ldx, w, K, sms, stream) : lf_launch<false, false, KIND>(p, x, ldx, w, K, sms, stream);
     };
     if (!whole) return go(std::integral_constant<int, LF_ANY>());
     if (residual == nullptr) return e.out_bf16 ? go(std::integral_constant<int, LF_BF16>()) : go(std::integral_constant<int, LF_F32>());
     return e.out_bf16 ? go(std::integral_constant<int, LF_BF16_RES>()) : go(std::integral_constant<int, LF_F32_RES>());
 }
 
-// Partial sums of a row (8 bytes each) that a call leaves; form as above (0: the one chosen), ks 1.
-static int lf_score_form(int T, int N, int form, bool * pair) {
+// Partial sums of a row (8 bytes each) that a call leaves; form as above (0: the one chosen), ks 1, any bn where w's rows are the product's.
+static int lf_score_form(int T, int N, int form, bool * pair, bool * swap) {
     const int sms = lf_sms();
     *pair = T > TC_BM;
+    *swap = !*pair;          // (61 rows of x behind 4,096: 213 us, x's rows as the product's 237)
     if (form != 0) {
         *pair = form & 1;
-        return (form >> 1) & 0x7fff;
+        *swap = form >> 14 & 1;
+        const int bn = (form >> 1) & 0x1fff, step = *pair ? 32 : *swap ? 1 : 16;
+        return (*swap && (*pair || T > TC_BM || bn > TC_BM)) || bn < 32 || bn > 256 || bn % step != 0 ? 0 : bn;
     }
-    const int m_tiles = (T + (*pair ? 256 : 128) - 1) / (*pair ? 256 : 128), units = *pair ? sms / 2 : sms;
+    const int m_tiles = (T + (*pair ? 256 : 128) - 1) / (*pair ? 256 : 128), units = *pair ? sms / 2 : sms, most = *swap ? TC_BM : 256;
     if (*pair && m_tiles > 8) return 256;
-    const long long waves = std::max<long long>(1, ((long long) m_tiles * ((N + 255) / 256) + units - 1) / units);
-    return std::min(256, lf_even(N, (int) std::min<long long>(N, waves * units / m_tiles), *pair ? 32 : 16));
+    const long long waves = std::max<long long>(1, ((long long) m_tiles * ((N + most - 1) / most) + units - 1) / units);
+    return std::min(most, lf_even(N, (int) std::min<long long>(N, waves * units / m_tiles), *pair ? 32 : *swap ? 1 : 16));
 }
 IIAN_API int iian_linear_logprobs_tiles(int T, int N, int form) {
     if (T <= 0 || N <= 0) return 0;
-    bool pair;
-    const int bn = lf_score_form(T, N, form, &pair);
-    return bn < 32 ? 0 : 2 * ((N + bn - 1) / bn);
+    bool pair, swap;
+    const int bn = lf_score_form(T, N, form, &pair, &swap);
+    return bn < 32 ? 0 : (swap ? 4 : 2) * ((N + bn - 1) / bn);
 }
 
 // targets [T]; lp, lse [T] float32; part: [tiles][T] pairs of floats, tiles as iian_linear_logprobs_tiles says.
@@ -726,16 +855,17 @@ IIAN_API int iian_linear_logprobs(const void * x, long long ldx, const void * w,
     if (part == nullptr || cap < 0.0f) return IIAN_ERR_SHAPE;
     LfArgs p = {};
     const int sms = lf_sms();
-    bool pair;
+    bool pair, swap;
     p.T = T; p.N = N;
-    p.bn = lf_score_form(T, N, form, &pair);
+    p.bn = lf_score_form(T, N, form, &pair, &swap);
     p.ks = 1;
-    if (p.bn < 32 || p.bn > 256 || p.bn % (pair ? 32 : 16) != 0) return IIAN_ERR_SHAPE;
+    if (p.bn < 32) return IIAN_ERR_SHAPE;
     p.status = (TcStatus *) status;
     p.score = {(float2 *) part, targets, lp, cap};
-    rc = pair ? lf_launch<true, LF_SCORE>(p, x, ldx, w, K, sms, stream) : lf_launch<false, LF_SCORE>(p, x, ldx, w, K, sms, stream);
+    rc = pair ? lf_launch<true, false, LF_SCORE>(p, x, ldx, w, K, sms, stream)
+       : swap ? lf_launch<false, true, LF_SCORE>(p, x, ldx, w, K, sms, stream) : lf_launch<false, false, LF_SCORE>(p, x, ldx, w, K, sms, stream);
     if (rc != IIAN_OK) return rc;
-    return lf_join(part, 2 * ((N + p.bn - 1) / p.bn), T, N, targets, lp, lse, stream);
+    return lf_join(part, (swap ? 4 : 2) * ((N + p.bn - 1) / p.bn), T, N, targets, lp, lse, stream);
 }
 
 // The same from logits in memory, a piece of the vocabulary at a time: logits [T, P] float32 hold columns v0 .. v0 + P, whose `splits` parts

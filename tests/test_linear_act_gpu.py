@@ -87,6 +87,21 @@ def test_every_form(n, pair, bn, ks):
     check(n, 1048, 701, BF, BF, "silu", True, False, form(pair, bn, ks))          # entries, not groups of four
 
 
+@pytest.mark.parametrize("n", [1, 16, 61, 100, 128])
+@pytest.mark.parametrize("bn,ks", [(32, 1), (48, 8), (64, 2), (96, 3), (112, 6), (128, 1), (128, 4)])
+def test_every_form_of_few_rows(n, bn, ks):
+    check(n, 1048, 700, BF, F32, "relu", True, True, form(0, bn, ks) | 1 << 14)
+    check(n, 1048, 701, BF, BF, "silu", True, False, form(0, bn, ks) | 1 << 14)
+    check(n, 72, 36, BF, F32, "none", True, True, form(0, bn, min(ks, 2)) | 1 << 14)
+
+
+@pytest.mark.parametrize("n,bn", [(4, 144), (129, 64)])
+def test_few_rows_are_few(n, bn):
+    x, w, out = (torch.zeros(s, device="cuda", dtype=BF) for s in ((n, 1024), (64, 1024), (n, 64)))
+    with pytest.raises(KernelError):
+        K().linear_act(x, w, out, form=form(0, bn, 1) | 1 << 14)
+
+
 @pytest.mark.parametrize("bad", [(0, 16, 1), (0, 40, 1), (0, 272, 1), (1, 48, 1), (0, 64, 9), (1, 64, 5), (0, 64, 0), (0, 32, 8 + 1)])
 def test_forms_there_are_none_of(bad):
     x, w, out = (torch.zeros(s, device="cuda", dtype=BF) for s in ((4, 1024), (64, 1024), (4, 64)))
@@ -109,6 +124,10 @@ def test_rows_apart_and_what_lies_between_them(dtype, n, k, m):
     untouched = wide_o.clone()
     untouched[:n, 4:4 + m] = 7.0
     assert (untouched == 7.0).all()
+    x = wide_x[:n, 4:4 + k]                                         # rows that do not begin on 16 bytes
+    K().linear_act(x, w, out, activation="gelu", residual=r)
+    y, ref = reference(x, w, None, "gelu", r)
+    assert ((out.double() - ref).abs() <= tolerance(x, w, y, ref, "gelu", F32, False)).all()
     one = wide_r[:1, 4:4 + m].expand(n, m)                         # one row for all of them
     K().linear_act(x, w, out, activation="gelu", residual=one)
     y, ref = reference(x, w, None, "gelu", one)

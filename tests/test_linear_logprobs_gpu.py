@@ -83,6 +83,19 @@ def test_every_form(n, pair, bn):
     check(n, 264, 3001, form=form(pair, bn))
 
 
+@pytest.mark.parametrize("n", [1, 17, 60, 128])
+@pytest.mark.parametrize("bn", [32, 57, 115, 128])
+def test_every_form_of_few_rows(n, bn):
+    check(n, 264, 3001, form=form(0, bn) | 1 << 14)
+    check(n, 264, 3001, cap=9.0, form=form(0, bn) | 1 << 14)
+
+
+@pytest.mark.parametrize("n,bad", [(4, 0 | 16 << 1), (4, 0 | 272 << 1), (4, 0 | 40 << 1), (300, 1 | 48 << 1), (4, 1 << 14 | 144 << 1), (200, 1 << 14 | 64 << 1)])
+def test_forms_there_are_none_of(n, bad):
+    with pytest.raises(KernelError):
+        check(n, 64, 500, form=bad | 1 << 16)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_more_rows_than_a_launch_takes(dtype, monkeypatch):
     monkeypatch.setattr(backend.CudaKernels, "SCORE_ROWS", 100)
