@@ -70,6 +70,18 @@ def test_float32(n, k, m):
     check(n, k, m, F32, F32, "none", False, False)
 
 
+@pytest.mark.parametrize("n,k,m", [(1, 4097, 130), (3, 1001, 64), (8, 77, 6150), (9, 258, 4100), (16, 31, 100), (16, 514, 6144), (17, 1023, 65), (84, 3199, 181),
+                                   (301, 515, 1030), (1025, 130, 2050)])
+def test_float32_rows_that_do_not_begin_on_16_bytes(n, k, m):
+    check(n, k, m, F32, F32, "silu", True, True)
+    check(n, k, m, F32, F32, "none", False, False)
+    wide = torch.randn(n, 4 * k + 3, device="cuda")                  # 4 k floats wide: every piece of a row but its place is whole
+    x, w, out = wide[:, 1:1 + 4 * k], torch.randn(m, 4 * k, device="cuda") * 0.05, torch.empty(n, m, device="cuda")
+    K().linear_act(x, w, out)
+    y, ref = reference(x, w, None, "none", None)
+    assert ((out.double() - ref).abs() <= tolerance(x, w, y, ref, "none", F32, False)).all()
+
+
 @pytest.mark.parametrize("dtype,wdtype,k", [(BF, F32, 64), (F32, BF, 64), (BF, BF, 71), (BF, BF, 4)])
 def test_what_the_tensor_cores_do_not_take(dtype, wdtype, k):
     check(33, k, 50, dtype, BF, "relu", True, True, wdtype=wdtype)
