@@ -378,9 +378,9 @@ static int launch_rows(const float * x, const float * w, TO * out, int N, int M,
     return iian_launch_status();
 }
 
-// Up to kRowsMax rows the streaming form; its CTAs own 32 weight rows where there are enough of them for every SM, 8 below
-// (us: 2 x 6,144 x 1,024 14.3 against 16.5; 16 x 4,096 x 4,096 67 against 96; but 4 x 4,096 x 12,288 113 against 76, 12 x 1,024 x 1,024
-// 18.7 against 10.8).  Above, the tile that makes the fullest SM finish first; us:
+// Up to 8 rows the streaming form, and up to kRowsMax where there are fewer than 4,096 columns (9 x 12,288 x 4,096: 107 us against the ring's
+// 72); its CTAs own 32 weight rows where there are enough of them for every SM, 8 below (us: 2 x 6,144 x 1,024 14.3 against 16.5; 4 x 4,096 x
+// 12,288 113 against 76, 12 x 1,024 x 1,024 18.7 against 10.8).  Above, the tile that makes the fullest SM finish first; us:
 //   rows x columns x K     64 x 128   64 x 64 (8 x 4)   ring: 32 x 64   32 x 32   16 x 32   the plain form
 //   301 x 4,096 x 1,024       108            87               78            82        99         156
 //   301 x 1,024 x 2,048       127            76               76            56        58         157
@@ -393,14 +393,15 @@ static int launch_rows(const float * x, const float * w, TO * out, int N, int M,
 //   256 x 4,096 x 1,024        70            64               70            82        84
 //   1,024 x 1,024 x 3,072     189           177              189           223       234
 //   2,048 x 6,144 x 4,096   2,023         2,107                                                3,996
-// Rows that do not begin on 16 bytes (PIECE 1) come a float at a time, and only into rings; us, beside the plain form's and those of one more of K:
-//   4 x 12,288 x 4,095 109 (545, 62), 17 x 4,096 x 1,023 25 (80, 20), 120 x 1,024 x 2,047 41 (159, 35), 1,024 x 4,096 x 4,095 1,032 (1,377, 759)
+// A ring of 24 x 32 besides: 301 x 1,024 x 2,048 49, 24 x 4,096 x 4,096 52 (16 x 32: 60), 33 x 2,196 x 5,232 61 (16 x 32: 78).
+// Rows that do not begin on 16 bytes (PIECE 1) come a float at a time, and only into rings, up to 2 rows into the streaming form's; us,
+// beside the plain form's and those of one less of K:
+//   4 x 12,288 x 4,097 99 (545, 62), 17 x 1,024 x 1,025 17 (78, 12), 200 x 1,024 x 2,049 44 (160, 38), 1,024 x 4,096 x 4,097 1,016 (1,377, 733)
 template <int PIECE, typename TO, typename EPI>
 static int launch_f32(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
-    if (N <= kRowsMax) {
+    if (PIECE == 4 ? N <= 8 || (N <= kRowsMax && M < 4096) : N <= 2) {
         if (M < (N > 8 ? 4096 : 6144)) return launch_rows<8, 6, 1, PIECE>(x, w, out, N, M, K, epi, stream);
-        if (N <= 4) return launch_rows<32, 3, 1, PIECE>(x, w, out, N, M, K, epi, stream);
-        return N <= 8 ? launch_rows<32, 3, 2, PIECE>(x, w, out, N, M, K, epi, stream) : launch_rows<32, 3, 4, PIECE>(x, w, out, N, M, K, epi, stream);
+        return N <= 4 ? launch_rows<32, 3, 1, PIECE>(x, w, out, N, M, K, epi, stream) : launch_rows<32, 3, 2, PIECE>(x, w, out, N, M, K, epi, stream);
     }
     // us per 1,024 of K: `alone` for the first tile of an SM, `more` for each further one that runs beside it (up to `beside`), `then` for
     // those that wait for one of them to end
@@ -411,14 +412,16 @@ static int launch_f32(const float * x, const float * w, TO * out, int N, int M, 
     };
     const double wide = PIECE == 4 ? cost(64, 128, 65.0, 43.0, 1, 43.0) : 1e30, even = PIECE == 4 ? cost(64, 64, 45.0, 13.5, 1, 26.0) : 1e30;
     const double half = cost(32, 64, 24.5, 12.0, 2, 14.8), small = cost(32, 32, 15.0, 7.7, 2, 9.2), least = cost(16, 32, 11.5, 4.1, 2, 5.5);
-    const double best = std::min({wide, even, half, small, least});
+    const double three = cost(24, 32, 12.2, 5.4, 2, 8.5);
+    const double best = std::min({wide, even, half, small, three, least});
     if constexpr (PIECE == 4) {
         if (wide == best) return launch_tile<64, 128, 8, 8, 1>(x, w, out, N, M, K, epi, stream);
         if (even == best) return launch_tile<64, 64, 8, 4, 3>(x, w, out, N, M, K, epi, stream);
     }
     if (half == best) return launch_ring<4, 4, 3, 32, PIECE>(x, w, out, N, M, K, epi, stream);
     if (small == best) return launch_ring<4, 2, 4, 64, PIECE>(x, w, out, N, M, K, epi, stream);
-    return launch_ring<2, 2, 4, 32, PIECE>(x, w, out, N, M, K, epi, stream);
+    if (three == best) return launch_ring<3, 2, 4, 64, PIECE>(x, w, out, N, M, K, epi, stream);
+    return launch_ring<2, 2, 4, PIECE == 4 ? 32 : 64, PIECE>(x, w, out, N, M, K, epi, stream);
 }
 
 template <typename TX, typename TW, typename TO, typename EPI>
