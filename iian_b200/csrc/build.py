@@ -33,14 +33,14 @@ SOURCE_HEADERS: Dict[str, List[str]] = {"attention_mma": ["paged_mma.cuh"], "dif
                                          "gemm_tcgen05": ["gated.cuh", "tc_product.cuh"], "attention_tc": ["tc_attention.cuh", "packed.cuh"],
                                          "latent_attention_tc": ["tc_attention.cuh", "packed.cuh", "latent_merge.cuh"],
                                          "latent_attention_mma": ["latent_merge.cuh"], "gemm_simt": ["packed.cuh", "epilogue.cuh"],
-                                         "linear_fused": ["epilogue.cuh", "tc_product.cuh"],
+                                         "linear_fused": ["epilogue.cuh", "tc_product.cuh"], "linear_f32": ["epilogue.cuh", "packed.cuh", "tc_product.cuh"],
                                          "attention_generic": ["packed.cuh"], "delta_rule": ["packed.cuh"]}
 
 # every library of the engine; build_all() compiles them all
 SOURCES = ["elementwise", "rope_kv", "attention_generic", "gemm_simt", "sampling", "gemm_skinny", "attention_mma", "prefetch", "gemm_tcgen05",
            "attention_tc", "gemm_stream", "postnorm", "latent_attention", "moe", "latent_attention_mma", "latent_attention_tc",
            "stream_ops", "shared_kv", "matrix_memory", "residual_ops", "chunked_attention", "delta_rule", "window_attention",
-           "decay_scan", "tanh_norm", "difference_attention", "difference_attention_mma", "moe_groups", "linear_fused"]
+           "decay_scan", "tanh_norm", "difference_attention", "difference_attention_mma", "moe_groups", "linear_fused", "linear_f32"]
 # libraries only the bfloat16 serving path uses
 BF16_SOURCES: List[str] = ["gemm_skinny", "attention_mma", "prefetch", "gemm_tcgen05", "attention_tc", "gemm_stream"]
 BF16_PRODUCT_SOURCES: List[str] = ["gemm_skinny", "gemm_tcgen05", "gemm_stream"]

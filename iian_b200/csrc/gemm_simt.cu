@@ -20,12 +20,6 @@ namespace iian {
 
 constexpr int BM = 64, BN = 64, BK = 16;
 
-// PIECE floats to shared memory, zeros where there are none
-template <int PIECE> __device__ __forceinline__ void copy_piece(float * to, const float * from, bool there) {
-    if constexpr (PIECE == 4) copy16(to, from, there);
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned) __cvta_generic_to_shared(to)), "l"(from), "r"(there ? 4 : 0));
-}
-
 // What becomes of a sum, and how far apart the rows of x are: the product itself goes to `out` ...
 struct Plain { static constexpr bool fused = false; };
 // ... or with bias, activation and residual (epilogue.cuh) to where that says
@@ -101,9 +95,9 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const TX * __restrict__ 
 // multiply-adds).  The loader's 16-byte pieces along k are put down as four words in four rows, the column flipped by 8 in the upper
 // half of a stage so that a warp's words fall into 32 banks.  2,048 x 6,144 x 4,096: 2,023 us (51 TFLOP/s; 4 x 4 blocks without
 // packing 3,996 us).
-template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO, typename EPI>
+template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO>
 __global__ void __launch_bounds__((TILE_N / TN) * (TILE_M / TM))
-gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
+gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K) {
     constexpr int THREADS = (TILE_N / TN) * (TILE_M / TM), TX = TILE_M / TM;
     constexpr int LX = TILE_N * BK / 4 / THREADS, LW = TILE_M * BK / 4 / THREADS;        // 16-byte pieces a thread loads per stage
     static_assert(LX * THREADS * 4 == TILE_N * BK && LW * THREADS * 4 == TILE_M * BK && BK == 16, "whole pieces per thread");
@@ -111,7 +105,6 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
     __shared__ __align__(16) float ws[2][BK][TILE_M + 4];
     const int tid = threadIdx.x, tx = tid % TX, ty = tid / TX;
     const int n0 = blockIdx.y * TILE_N, m0 = blockIdx.x * TILE_M;
-    const int ldx = row_distance(epi, K);
     unsigned long long acc[TN][TM / 2];
 #pragma unroll
     for (int i = 0; i < TN; i++)
@@ -124,7 +117,7 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 #pragma unroll
         for (int i = 0; i < LX; i++) {
             const int n = n0 + (tid + i * THREADS) / 4;
-            px[i] = n < N && k < K ? __ldg(reinterpret_cast<const float4 *>(x + (size_t) n * ldx + k)) : zero;
+            px[i] = n < N && k < K ? __ldg(reinterpret_cast<const float4 *>(x + (size_t) n * K + k)) : zero;
         }
 #pragma unroll
         for (int i = 0; i < LW; i++) {
@@ -190,8 +183,8 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
         for (int j = 0; j < TM / 2; j++) {
             const int m = m0 + (j / 2) * (TILE_M / (TM / 4)) + tx * 4 + (j % 2) * 2;
             const float2 v = unpack2(acc[i][j]);
-            if (m < M) put_out(out, epi, n, m, M, v.x);
-            if (m + 1 < M) put_out(out, epi, n, m + 1, M, v.y);
+            if (m < M) out[(size_t) n * M + m] = from_f32<TO>(v.x);
+            if (m + 1 < M) out[(size_t) n * M + m + 1] = from_f32<TO>(v.y);
         }
     }
 }
@@ -202,21 +195,19 @@ gemm_tile_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 // Lanes are dealt so that neighbours share a row of one operand or of the other (bits 0 and 4 pick the row of x, bits 1 to 3 that of w):
 // 16-byte reads then take 2 clocks a warp, 4 where equal addresses lie 8 lanes apart.  What bounds it: one warp a scheduler leaves
 // the 4-clock chain and the reads' latency bare, more of them the dispatch of three-operand multiply-adds (41 clocks for 32).
-// PIECE: the floats of one copy, 4 or, where rows do not begin on 16 bytes, 1.
-template <int TN, int TM, int WY, int WX, int STAGES, int DEPTH, int PIECE, typename TO, typename EPI>
+template <int TN, int TM, int WY, int WX, int STAGES, int DEPTH, typename TO>
 __global__ void __launch_bounds__(WY * WX * 32)
-gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
-    constexpr int TILE_N = 4 * TN * WY, TILE_M = 8 * TM * WX, THREADS = WY * WX * 32, LD = DEPTH + 4, PIECES = DEPTH / PIECE;
+gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K) {
+    constexpr int TILE_N = 4 * TN * WY, TILE_M = 8 * TM * WX, THREADS = WY * WX * 32, LD = DEPTH + 4, PIECES = DEPTH / 4;
     constexpr int LOADS = (TILE_N + TILE_M) * PIECES / THREADS;
     static_assert(LOADS * THREADS == (TILE_N + TILE_M) * PIECES && THREADS % PIECES == 0, "whole pieces per thread");
     extern __shared__ __align__(16) float ring[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n0 = blockIdx.y * TILE_N, m0 = blockIdx.x * TILE_M;
-    const int ldx = row_distance(epi, K);
     const int turns = (K + DEPTH - 1) / DEPTH;
     auto fill = [&](int s) {
         if (s < turns) {
-            const int at = tid % PIECES * PIECE, k = s * DEPTH + at;     // K is a multiple of PIECE: a piece lies inside or outside as a whole
+            const int at = tid % PIECES * 4, k = s * DEPTH + at; // K is a multiple of 4: a piece lies inside or outside as a whole
             float * to = ring + (s % STAGES) * (TILE_N + TILE_M) * LD + at;
 #pragma unroll
             for (int i = 0; i < LOADS; i++) {
@@ -224,7 +215,7 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
                 const bool is_x = r < TILE_N;
                 const int g = is_x ? n0 + r : m0 + r - TILE_N;
                 const bool in = k < K && g < (is_x ? N : M);
-                copy_piece<PIECE>(to + r * LD, in ? (is_x ? x : w) + (size_t) g * (is_x ? ldx : K) + k : x, in);
+                copy16(to + r * LD, in ? (is_x ? x : w) + (size_t) g * K + k : x, in);
             }
         }
         asm volatile("cp.async.commit_group;");
@@ -275,7 +266,7 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 #pragma unroll
         for (int j = 0; j < TM; j++) {
             const int m = m0 + col + 8 * j;
-            if (m < M) put_out(out, epi, n, m, M, acc[i][j]);
+            if (m < M) out[(size_t) n * M + m] = from_f32<TO>(acc[i][j]);
         }
     }
 }
@@ -287,25 +278,24 @@ gemm_ring_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 // 2 x 1,024 x 3,072: 20 us (210 us).
 constexpr int kRowsThreads = 128, kRowsK = 128, kRowsMax = 16;
 
-template <int TILE_M, int STAGES, int PER, int PIECE, typename TO, typename EPI>
+template <int TILE_M, int STAGES, int PER, typename TO>
 __global__ void __launch_bounds__(kRowsThreads)
-gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K, const EPI epi) {
+gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, TO * __restrict__ out, int N, int M, int K) {
     constexpr int LD = kRowsK + 4, GROUPS = kRowsThreads / TILE_M;       // rows 4 banks apart: 16-byte reads of 8 lanes hit 32 banks
     extern __shared__ __align__(16) float ring[];
     const int stage_floats = (TILE_M + N) * LD;
-    const int ldx = row_distance(epi, K);
     const int tid = threadIdx.x, m0 = blockIdx.x * TILE_M, m = tid % TILE_M, g = tid / TILE_M;
     const int turns = (K + kRowsK - 1) / kRowsK;
     auto fill = [&](int s) {
         if (s < turns) {
             float * to = ring + (s % STAGES) * stage_floats;
             const int k0 = s * kRowsK;
-            for (int e = tid; e < (TILE_M + N) * (kRowsK / PIECE); e += kRowsThreads) {
-                const int r = e / (kRowsK / PIECE), k = k0 + (e % (kRowsK / PIECE)) * PIECE;
+            for (int e = tid; e < (TILE_M + N) * (kRowsK / 4); e += kRowsThreads) {
+                const int r = e / (kRowsK / 4), k = k0 + (e % (kRowsK / 4)) * 4;
                 const bool is_w = r < TILE_M;
                 const bool in = k < K && (!is_w || m0 + r < M);
-                const float * from = is_w ? w + (size_t) (m0 + r) * K + k : x + (size_t) (r - TILE_M) * ldx + k;
-                copy_piece<PIECE>(to + r * LD + (k - k0), in ? from : x, in);
+                const float * from = is_w ? w + (size_t) (m0 + r) * K + k : x + (size_t) (r - TILE_M) * K + k;
+                copy16(to + r * LD + (k - k0), in ? from : x, in);
             }
         }
         asm volatile("cp.async.commit_group;");
@@ -340,41 +330,38 @@ gemm_rows_kernel(const float * __restrict__ x, const float * __restrict__ w, TO 
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int n = g + i * GROUPS;
-        if (n < N && m0 + m < M) {
-            if constexpr (EPI::fused) epi.e.store(acc[i], (size_t) n, m0 + m);
-            else out[(size_t) n * M + m0 + m] = from_f32<TO>(acc[i]);
-        }
+        if (n < N && m0 + m < M) out[(size_t) n * M + m0 + m] = from_f32<TO>(acc[i]);
     }
 }
 
-template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO, typename EPI>
-static int launch_tile(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
+template <int TILE_N, int TILE_M, int TN, int TM, int AHEAD, typename TO>
+static int launch_tile(const float * x, const float * w, TO * out, int N, int M, int K, cudaStream_t stream) {
     const dim3 grid((M + TILE_M - 1) / TILE_M, (N + TILE_N - 1) / TILE_N);
-    gemm_tile_kernel<TILE_N, TILE_M, TN, TM, AHEAD, TO, EPI><<<grid, (TILE_N / TN) * (TILE_M / TM), 0, stream>>>(x, w, out, N, M, K, epi);
+    gemm_tile_kernel<TILE_N, TILE_M, TN, TM, AHEAD, TO><<<grid, (TILE_N / TN) * (TILE_M / TM), 0, stream>>>(x, w, out, N, M, K);
     return iian_launch_status();
 }
 
-template <int TN, int TM, int STAGES, int DEPTH, int PIECE, typename TO, typename EPI>
-static int launch_ring(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
+template <int TN, int TM, int STAGES, int DEPTH, typename TO>
+static int launch_ring(const float * x, const float * w, TO * out, int N, int M, int K, cudaStream_t stream) {
     constexpr int TILE_N = 8 * TN, TILE_M = 16 * TM;         // two by two warps
     constexpr size_t smem = (size_t) STAGES * (TILE_N + TILE_M) * (DEPTH + 4) * sizeof(float);
-    auto kernel = gemm_ring_kernel<TN, TM, 2, 2, STAGES, DEPTH, PIECE, TO, EPI>;
+    auto kernel = gemm_ring_kernel<TN, TM, 2, 2, STAGES, DEPTH, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
     if (e != cudaSuccess) return 1000 + (int) e;
     const dim3 grid((M + TILE_M - 1) / TILE_M, (N + TILE_N - 1) / TILE_N);
-    kernel<<<grid, 128, smem, stream>>>(x, w, out, N, M, K, epi);
+    kernel<<<grid, 128, smem, stream>>>(x, w, out, N, M, K);
     return iian_launch_status();
 }
 
-template <int TILE_M, int STAGES, int PER, int PIECE, typename TO, typename EPI>
-static int launch_rows(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
+template <int TILE_M, int STAGES, int PER, typename TO>
+static int launch_rows(const float * x, const float * w, TO * out, int N, int M, int K, cudaStream_t stream) {
     const size_t smem = (size_t) STAGES * (TILE_M + N) * (kRowsK + 4) * sizeof(float);
-    auto kernel = gemm_rows_kernel<TILE_M, STAGES, PER, PIECE, TO, EPI>;
+    auto kernel = gemm_rows_kernel<TILE_M, STAGES, PER, TO>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
         if (e != cudaSuccess) return 1000 + (int) e;
     }
-    kernel<<<(M + TILE_M - 1) / TILE_M, kRowsThreads, smem, stream>>>(x, w, out, N, M, K, epi);
+    kernel<<<(M + TILE_M - 1) / TILE_M, kRowsThreads, smem, stream>>>(x, w, out, N, M, K);
     return iian_launch_status();
 }
 
@@ -394,14 +381,11 @@ static int launch_rows(const float * x, const float * w, TO * out, int N, int M,
 //   1,024 x 1,024 x 3,072     189           177              189           223       234
 //   2,048 x 6,144 x 4,096   2,023         2,107                                                3,996
 // A ring of 24 x 32 besides: 301 x 1,024 x 2,048 49, 24 x 4,096 x 4,096 52 (16 x 32: 60), 33 x 2,196 x 5,232 61 (16 x 32: 78).
-// Rows that do not begin on 16 bytes (PIECE 1) come a float at a time, and only into rings, up to 2 rows into the streaming form's; us,
-// beside the plain form's and those of one less of K:
-//   4 x 12,288 x 4,097 99 (545, 62), 17 x 1,024 x 1,025 17 (78, 12), 200 x 1,024 x 2,049 44 (160, 38), 1,024 x 4,096 x 4,097 1,016 (1,377, 733)
-template <int PIECE, typename TO, typename EPI>
-static int launch_f32(const float * x, const float * w, TO * out, int N, int M, int K, const EPI & epi, cudaStream_t stream) {
-    if (PIECE == 4 ? N <= 8 || (N <= kRowsMax && M < 4096) : N <= 2) {
-        if (M < (N > 8 ? 4096 : 6144)) return launch_rows<8, 6, 1, PIECE>(x, w, out, N, M, K, epi, stream);
-        return N <= 4 ? launch_rows<32, 3, 1, PIECE>(x, w, out, N, M, K, epi, stream) : launch_rows<32, 3, 2, PIECE>(x, w, out, N, M, K, epi, stream);
+template <typename TO>
+static int launch_f32(const float * x, const float * w, TO * out, int N, int M, int K, cudaStream_t stream) {
+    if (N <= 8 || (N <= kRowsMax && M < 4096)) {
+        if (M < (N > 8 ? 4096 : 6144)) return launch_rows<8, 6, 1, TO>(x, w, out, N, M, K, stream);
+        return N <= 4 ? launch_rows<32, 3, 1, TO>(x, w, out, N, M, K, stream) : launch_rows<32, 3, 2, TO>(x, w, out, N, M, K, stream);
     }
     // us per 1,024 of K: `alone` for the first tile of an SM, `more` for each further one that runs beside it (up to `beside`), `then` for
     // those that wait for one of them to end
@@ -410,18 +394,16 @@ static int launch_f32(const float * x, const float * w, TO * out, int N, int M, 
         const long long tiles = (long long) ((N + tn - 1) / tn) * ((M + tm - 1) / tm), further = (tiles - 1) / 148;
         return alone + more * (double) std::min<long long>(further, beside) + then * (double) std::max<long long>(further - beside, 0);
     };
-    const double wide = PIECE == 4 ? cost(64, 128, 65.0, 43.0, 1, 43.0) : 1e30, even = PIECE == 4 ? cost(64, 64, 45.0, 13.5, 1, 26.0) : 1e30;
+    const double wide = cost(64, 128, 65.0, 43.0, 1, 43.0), even = cost(64, 64, 45.0, 13.5, 1, 26.0);
     const double half = cost(32, 64, 24.5, 12.0, 2, 14.8), small = cost(32, 32, 15.0, 7.7, 2, 9.2), least = cost(16, 32, 11.5, 4.1, 2, 5.5);
     const double three = cost(24, 32, 12.2, 5.4, 2, 8.5);
     const double best = std::min({wide, even, half, small, three, least});
-    if constexpr (PIECE == 4) {
-        if (wide == best) return launch_tile<64, 128, 8, 8, 1>(x, w, out, N, M, K, epi, stream);
-        if (even == best) return launch_tile<64, 64, 8, 4, 3>(x, w, out, N, M, K, epi, stream);
-    }
-    if (half == best) return launch_ring<4, 4, 3, 32, PIECE>(x, w, out, N, M, K, epi, stream);
-    if (small == best) return launch_ring<4, 2, 4, 64, PIECE>(x, w, out, N, M, K, epi, stream);
-    if (three == best) return launch_ring<3, 2, 4, 64, PIECE>(x, w, out, N, M, K, epi, stream);
-    return launch_ring<2, 2, 4, PIECE == 4 ? 32 : 64, PIECE>(x, w, out, N, M, K, epi, stream);
+    if (wide == best) return launch_tile<64, 128, 8, 8, 1, TO>(x, w, out, N, M, K, stream);
+    if (even == best) return launch_tile<64, 64, 8, 4, 3, TO>(x, w, out, N, M, K, stream);
+    if (half == best) return launch_ring<4, 4, 3, 32, TO>(x, w, out, N, M, K, stream);
+    if (small == best) return launch_ring<4, 2, 4, 64, TO>(x, w, out, N, M, K, stream);
+    if (three == best) return launch_ring<3, 2, 4, 64, TO>(x, w, out, N, M, K, stream);
+    return launch_ring<2, 2, 4, 32, TO>(x, w, out, N, M, K, stream);
 }
 
 template <typename TX, typename TW, typename TO, typename EPI>
@@ -442,8 +424,8 @@ IIAN_API int iian_gemm_simt(const void * x, int x_dtype, const void * w, int w_d
     if ((M + BM - 1) / BM > 2147483647 || (N + BN - 1) / BN > 65535) return IIAN_ERR_LIMIT;
     typedef __nv_bfloat16 bf;
     if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32 && K % 4 == 0 && ((uintptr_t) x | (uintptr_t) w) % 16 == 0)
-        return out_dtype == IIAN_F32 ? launch_f32<4>((const float *) x, (const float *) w, (float *) out, N, M, K, Plain(), stream)
-             : out_dtype == IIAN_BF16 ? launch_f32<4>((const float *) x, (const float *) w, (bf *) out, N, M, K, Plain(), stream) : (int) IIAN_ERR_DTYPE;
+        return out_dtype == IIAN_F32 ? launch_f32((const float *) x, (const float *) w, (float *) out, N, M, K, stream)
+             : out_dtype == IIAN_BF16 ? launch_f32((const float *) x, (const float *) w, (bf *) out, N, M, K, stream) : (int) IIAN_ERR_DTYPE;
     const int key = x_dtype * 4 + w_dtype * 2 + out_dtype;
     switch (key) {
         case 0: return launch<float, float, float>(x, w, out, N, M, K, Plain(), stream);
@@ -458,7 +440,8 @@ IIAN_API int iian_gemm_simt(const void * x, int x_dtype, const void * w, int w_d
     return IIAN_ERR_DTYPE;
 }
 
-// The product with bias, activation and residual (epilogue.cuh); x rows ldx apart.  The products and sums are those of the plain product.
+// The product with bias, activation and residual (epilogue.cuh); x rows ldx apart: for operands that are not
+// both float32, nor both bfloat16 with rows that the tensor cores' product takes.
 IIAN_API int iian_linear_act_simt(const void * x, int x_dtype, long long ldx, const void * w, int w_dtype, const float * bias,
                                   const void * residual, int res_dtype, long long ldr, void * out, int out_dtype, long long ldo, int N, int M,
                                   int K, int act, cudaStream_t stream) {
@@ -469,11 +452,6 @@ IIAN_API int iian_linear_act_simt(const void * x, int x_dtype, long long ldx, co
     Fused f = {};
     if (!linear_epilogue(f.e, bias, residual, res_dtype, ldr, out, out_dtype, ldo, act)) return IIAN_ERR_DTYPE;
     f.ldx = (int) ldx;
-    if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32 && K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t) x | (uintptr_t) w) % 16 == 0)
-        return launch_f32<4>((const float *) x, (const float *) w, (float *) nullptr, N, M, K, f, stream);
-    if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32 && (N + 31) / 32 <= 65535)
-        return launch_f32<1>((const float *) x, (const float *) w, (float *) nullptr, N, M, K, f, stream);
-    if (x_dtype == IIAN_F32 && w_dtype == IIAN_F32) return launch<float, float, float>(x, w, nullptr, N, M, K, f, stream);
     if (x_dtype == IIAN_F32 && w_dtype == IIAN_BF16) return launch<float, bf, float>(x, w, nullptr, N, M, K, f, stream);
     if (x_dtype == IIAN_BF16 && w_dtype == IIAN_F32) return launch<bf, float, float>(x, w, nullptr, N, M, K, f, stream);
     if (x_dtype == IIAN_BF16 && w_dtype == IIAN_BF16) return launch<bf, bf, float>(x, w, nullptr, N, M, K, f, stream);

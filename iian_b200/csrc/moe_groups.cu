@@ -412,11 +412,8 @@ IIAN_API int iian_moe_route_grouped(const float * logits, long long ld, const fl
     p.chunk = (per + p.lanes - 1) / p.lanes;
     const int vec = p.chunk % 4 == 0 && per % 4 == 0 && ld % 4 == 0 && (((uintptr_t) logits | (uintptr_t) correction) & 15) == 0;
     const dim3 grid((unsigned) (((long long) N + warps - 1) / warps));
-    auto go = [&](auto kernel) { return iian_launch(kernel, grid, dim3(warps * 32), 0, stream, p, N, vec); };
-    if (p.chunk <= 2) return go(moe_route_grouped_kernel<2>);
-    if (p.chunk <= 4) return go(moe_route_grouped_kernel<4>);
-    if (p.chunk <= 8) return go(moe_route_grouped_kernel<8>);
-    if (p.chunk <= 16) return go(moe_route_grouped_kernel<16>);
-    if (p.chunk <= 32) return go(moe_route_grouped_kernel<32>);
-    return go(moe_route_grouped_kernel<64>);                 // 17 groups of 60: half of the lanes hold nothing
+    auto kernel = p.chunk <= 2 ? moe_route_grouped_kernel<2> : p.chunk <= 4 ? moe_route_grouped_kernel<4> : p.chunk <= 8 ? moe_route_grouped_kernel<8>
+                : p.chunk <= 16 ? moe_route_grouped_kernel<16> : p.chunk <= 32 ? moe_route_grouped_kernel<32>
+                : moe_route_grouped_kernel<64>;              // 17 groups of 60: half of the lanes hold nothing
+    return iian_launch(kernel, grid, dim3(warps * 32), 0, stream, p, N, vec);
 }

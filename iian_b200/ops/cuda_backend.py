@@ -177,6 +177,7 @@ _MOE_ROUTE_GROUPED_ARGS = [c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, 
                            c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p]
 _LINEAR_ACT_ARGS = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int,
                     c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+_LINEAR_ACT_F32_ARGS = _LINEAR_ACT_ARGS[:-2] + [c_void_p]
 _LINEAR_ACT_SIMT_ARGS = [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
                          c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p]
 _LINEAR_LOGPROBS_TILES_ARGS = [c_int, c_int, c_int]
@@ -2382,7 +2383,7 @@ class CudaKernels:
         x [N, K] and w [M, K] float32 or bfloat16, ``bias`` float32 [M], ``residual`` and ``out`` [N, M] float32 or bfloat16 each; rows of x,
         residual and out may be apart.  ``residual`` may be ``out`` itself (the same tensor, or one of the same place, type and row distance);
         other than that out overlaps none of them.  ``activation``: ``none``, ``silu``, ``gelu_tanh``, ``gelu`` (by erf), ``relu``, ``relu2``.  ``form``: a
-        tile of the tensor cores' product other than the one it chooses (csrc/linear_fused.cu)."""
+        tile other than the one that is chosen (csrc/linear_fused.cu, linear_f32.cu)."""
         n, k, m, xp, ldx, wp, tc = self._product_rows(x, w, "linear_act")
         act = self.LINEAR_ACTIVATIONS.get(activation)
         if act is None:
@@ -2407,6 +2408,12 @@ class CudaKernels:
             fn = _entry("linear_fused", "iian_linear_act", _LINEAR_ACT_ARGS)
             _check(fn(xp, ldx, wp, bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, form, status, stream), "linear_act")
             return
+        if x.dtype == w.dtype == torch.float32:
+            fn = _entry("linear_f32", "iian_linear_act_f32", _LINEAR_ACT_F32_ARGS)
+            _check(fn(xp, ldx, wp, bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, form, stream), "linear_act_f32")
+            return
+        if form:
+            raise KernelError("linear_act: operands of these types and places have one form")
         fn = _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
         _check(fn(xp, _CODE[x.dtype], ldx, wp, _CODE[w.dtype], bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, stream), "linear_act_simt")
 
@@ -2454,12 +2461,16 @@ class CudaKernels:
         pieces = -(-v // width)
         logits = torch.empty(t * width, dtype=torch.float32, device=x.device)
         part = torch.empty(2 * pieces * splits * t, dtype=torch.float32, device=x.device)
-        product = _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
+        f32 = x.dtype == w.dtype == torch.float32
+        product = _entry("linear_f32", "iian_linear_act_f32", _LINEAR_ACT_F32_ARGS) if f32 else _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
         take = _entry("linear_fused", "iian_linear_logprobs_piece", _LINEAR_LOGPROBS_PIECE_ARGS)
         for i in range(pieces):
             v0, p = i * width, min(width, v - i * width)
-            _check(product(xp, _CODE[x.dtype], ldx, wp + v0 * k * w.element_size(), _CODE[w.dtype], 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k,
-                           0, stream), "linear_act_simt")
+            piece = wp + v0 * k * w.element_size()
+            if f32:
+                _check(product(xp, ldx, piece, 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k, 0, 0, stream), "linear_act_f32")
+            else:
+                _check(product(xp, _CODE[x.dtype], ldx, piece, _CODE[w.dtype], 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k, 0, stream), "linear_act_simt")
             _check(take(logits.data_ptr(), t, p, v0, at[0], at[1], part.data_ptr(), i * splits, splits, cap, stream), "linear_logprobs_piece")
         join = _entry("linear_fused", "iian_linear_logprobs_join", _LINEAR_LOGPROBS_JOIN_ARGS)
         _check(join(part.data_ptr(), pieces * splits, t, v, *at, stream), "linear_logprobs_join")

@@ -82,6 +82,20 @@ def test_float32_rows_that_do_not_begin_on_16_bytes(n, k, m):
     assert ((out.double() - ref).abs() <= tolerance(x, w, y, ref, "none", F32, False)).all()
 
 
+@pytest.mark.parametrize("tile", range(5))
+@pytest.mark.parametrize("ks", [1, 2, 3, 4, 6, 8])
+def test_every_form_of_float32(tile, ks):
+    for n, k, m in ((1, 1, 1), (3, 40, 33), (33, 1027, 65), (70, 516, 130), (9, 4096, 64)):
+        check(n, k, m, F32, F32, "gelu", True, True, form=tile + 1 | ks << 8)
+
+
+@pytest.mark.parametrize("bad", [6 | 1 << 8, 255 | 1 << 8, 1 << 8, 1, 1 | 9 << 8, -1])
+def test_forms_that_float32_has_not(bad):
+    x, w, out = (torch.zeros(s, device="cuda") for s in ((4, 64), (8, 64), (4, 8)))
+    with pytest.raises(KernelError):
+        K().linear_act(x, w, out, form=bad)
+
+
 @pytest.mark.parametrize("dtype,wdtype,k", [(BF, F32, 64), (F32, BF, 64), (BF, BF, 71), (BF, BF, 4)])
 def test_what_the_tensor_cores_do_not_take(dtype, wdtype, k):
     check(33, k, 50, dtype, BF, "relu", True, True, wdtype=wdtype)
