@@ -4,10 +4,11 @@
 // A warp holds the whole tile of its CTA, 4 TN rows of x by 8 TM rows of w, for a share of K: the blocks of 16 of K go round the warps of
 // the CTA and, where there are few tiles, of a cluster of CTAs, each warp with a ring of its own that it fills by cp.async and nobody else
 // waits for.  The warps' parts are added at the end, in their order, through shared memory and the cluster's.  So a thread has up to 8 x 8
-// sums although a CTA's tile is small enough for every SM to have some, and reads 16 bytes of shared memory per 16 multiply-adds.
+// sums although a CTA's tile is small enough for every SM to have some, and reads 16 bytes of shared memory per 16 multiply-adds.  What part
+// of K a warp has depends on K and on the rows of w: a row of x has the same bits whatever rows are beside it.
 // What bounds it: many rows, the packed multiply-adds, of which an SM takes some 60 % of what the pipe's width says, whatever feeds them (301 x
-// 2,048 x 1,024 45 us, of which 17.5 at the full width; the plain product's form with tiles that every warp shares 54); few rows, the
-// weights (1 x 12,288 x 4,096 45 us, 4.4 TB/s); few of everything, the latency of a ring's first turn and the join (1 x 155 x 9,596 10.3 us, one
+// 2,048 x 1,024 48 us, of which 17.5 at the full width; the plain product's form with tiles that every warp shares 54); few rows, the
+// weights (1 x 12,288 x 4,096 45 us, 4.4 TB/s); few of everything, the latency of a ring's first turn and the join (1 x 155 x 9,596 14 us, one
 // chain over K 49).
 // Each sum is a pair, of the even k and of the odd ones, so that packed multiply-adds take the operands as they lie in memory; a chain then is
 // K over twice the warps long, and rounds less than one over all of K.
@@ -113,16 +114,25 @@ linear_f32_kernel(const float * __restrict__ x, long long ldx, const float * __r
         if (epi.res != nullptr) { y[0] += d.x; y[1] += d.y; y[2] += d.z; y[3] += d.w; }
         epi.put4(y, (size_t) (n0 + r), m0 + c, live);
     };
+    constexpr int GROUPS = WARPS / 4;                        // four warps' parts first, then those of all groups in their order, whoever holds them
+    auto add = [](float4 & v, const float4 & u) { v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w; };
     for (int e = threadIdx.x; e < ROWS * COLS / 4; e += WARPS * 32) {
         const int r = e / (COLS / 4), c = e % (COLS / 4) * 4;
-        float4 v = *reinterpret_cast<const float4 *>(smem + r * PLD + c);
+        float4 v[GROUPS];
 #pragma unroll
-        for (int p = 1; p < WARPS; p++) {
-            const float4 u = *reinterpret_cast<const float4 *>(smem + (p * ROWS + r) * PLD + c);
-            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        for (int g = 0; g < GROUPS; g++) {
+            v[g] = *reinterpret_cast<const float4 *>(smem + (g * 4 * ROWS + r) * PLD + c);
+#pragma unroll
+            for (int p = 1; p < 4; p++) add(v[g], *reinterpret_cast<const float4 *>(smem + ((g * 4 + p) * ROWS + r) * PLD + c));
         }
-        if (ks > 1) *reinterpret_cast<float4 *>(smem + r * PLD + c) = v;
-        else put(r, c, v);
+        if (ks > 1) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) *reinterpret_cast<float4 *>(smem + (g * 4 * ROWS + r) * PLD + c) = v[g];
+        } else {
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++) add(v[0], v[g]);
+            put(r, c, v[0]);
+        }
     }
     if (ks > 1) {
         __syncthreads();
@@ -130,12 +140,16 @@ linear_f32_kernel(const float * __restrict__ x, long long ldx, const float * __r
         const unsigned base = (unsigned) __cvta_generic_to_shared(smem);
         for (int e = threadIdx.x + rank * WARPS * 32; e < ROWS * COLS / 4; e += ks * WARPS * 32) {
             const int r = e / (COLS / 4), c = e % (COLS / 4) * 4;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 v;
             for (int p = 0; p < ks; p++) {
-                float4 u;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(map_to_cta(base + (r * PLD + c) * 4, p)) : "memory");
-                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) {
+                    float4 u;
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w)
+                                 : "r"(map_to_cta(base + ((g * 4 * ROWS + r) * PLD + c) * 4, p)) : "memory");
+                    if (p == 0 && g == 0) v = u;
+                    else add(v, u);
+                }
             }
             put(r, c, v);
         }
@@ -163,26 +177,34 @@ static int ln_launch(const float * x, long long ldx, const float * w, int N, int
     return e == cudaSuccess ? iian_launch_status() : 1000 + (int) e;
 }
 
-// The tiles: rows of x, rows of w, and us as measured (1 to 2,048 rows, K 256 to 11,264): of a launch, per 1,024 of K for the first tile of
-// an SM and for each further one, of a tile's end, and of a cluster's join.  What is chosen by their sum is 3 % slower than the best on average.
-struct LnTile { int rows, cols; double launch, first, further, end, join; };
-constexpr LnTile LN_TILES[] = {{32, 64, 2.2, 18.2, 14.3, 1.6, 2.0}, {24, 64, 1.9, 15.1, 11.3, 1.6, 2.2}, {16, 64, 1.6, 13.0, 8.8, 1.6, 2.2},
-                               {16, 32, 2.1, 6.1, 4.6, 1.5, 1.5}, {8, 32, 1.8, 4.3, 3.2, 1.4, 2.2}};
+// Over how many groups of four warps K goes: by K and the rows of w alone, so that a row's sums are those of any other number of rows.  Few
+// rows of w leave SMs idle that could share K (1 x 155 x 9,596 14 us in eight groups, 38 in two), long K makes up for the join, short K does not
+// even for a second group's (1,300 x 1,500 x 700 86 us in one, 99 in two), unless there are few rows of w besides.
+static int ln_groups(int M, int K) {
+    if (K < 768) return M < 1024 ? 2 : 1;
+    return 2 * std::min(M < 1024 ? 4 : M < 4096 ? 2 : 1, K >= 4 * 768 ? 4 : K >= 2 * 768 ? 2 : 1);
+}
 
-static void ln_plan(int N, int M, int K, bool whole, int sms, int * tile, int * ks) {
-    static const int shares[] = {1, 2, 3, 4, 6, 8};
+// The tiles: rows of x, rows of w, warps, and us as measured (1 to 2,048 rows, K 256 to 11,264): of a launch, per 1,024 of K for the first
+// tile of an SM and for each further one, of a tile's end, and of a cluster's join.
+struct LnTile { int rows, cols, warps; double launch, first, further, end, join; };
+constexpr LnTile LN_TILES[] = {{32, 64, 4, 2.2, 18.2, 14.3, 1.6, 2.0}, {24, 64, 4, 1.9, 15.1, 11.3, 1.6, 2.2}, {16, 64, 4, 1.6, 13.0, 8.8, 1.6, 2.2},
+                               {16, 32, 8, 2.1, 6.1, 4.6, 1.5, 1.5}, {8, 32, 8, 1.8, 4.3, 3.2, 1.4, 2.2}};
+
+static int ln_plan(int N, int M, int K, int groups, int sms) {
+    int tile = 0;
     double best = 1e300;
     for (int v = 0; v < 5; v++) {
         const LnTile & p = LN_TILES[v];
-        const double tiles = (double) ((N + p.rows - 1) / p.rows) * ((M + p.cols - 1) / p.cols), k = (whole ? 1.0 : 1.15) * K / 1024.0;
-        for (int s : shares) {
-            if (s > 1 && (s * 128 > K || tiles * (s / 2) >= 4 * sms)) continue;
-            const double slots = s > 4 ? sms - sms / 9 : sms;            // clusters of six or eight leave some SMs of a GPC over
-            const double turns = std::ceil(tiles * s / slots);
-            const double t = p.launch + turns * p.end + k / s * (p.first + p.further * (turns - 1)) + (s > 1 ? p.join : 0.0);
-            if (t < best) { best = t; *tile = v; *ks = s; }
-        }
+        if (groups * 4 % p.warps != 0) continue;
+        const int ks = groups * 4 / p.warps;
+        const double tiles = (double) ((N + p.rows - 1) / p.rows) * ((M + p.cols - 1) / p.cols);
+        const double slots = ks > 4 ? sms - sms / 9 : sms;               // clusters of eight leave some SMs of a GPC over
+        const double turns = std::ceil(tiles * ks / slots);
+        const double t = p.launch + turns * p.end + K / 1024.0 / ks * (p.first + p.further * (turns - 1)) + (ks > 1 ? p.join : 0.0);
+        if (t < best) { best = t; tile = v; }
     }
+    return tile;
 }
 
 template <int PIECE>
@@ -201,7 +223,7 @@ static int ln_go(int tile, const float * x, long long ldx, const float * w, int 
 
 using namespace iian;
 
-// x rows ldx apart; form 0: the tile and the shares of K that suit the sizes, else tile + 1 | shares << 8
+// x rows ldx apart; form 0: the tile and the groups of warps that suit the sizes, else tile + 1 | groups << 8
 IIAN_API int iian_linear_act_f32(const float * x, long long ldx, const float * w, const float * bias, const void * residual, int res_dtype,
                                  long long ldr, void * out, int out_dtype, long long ldo, int N, int M, int K, int act, int form, cudaStream_t stream) {
     if (N <= 0 || M <= 0) return IIAN_OK;
@@ -211,8 +233,8 @@ IIAN_API int iian_linear_act_f32(const float * x, long long ldx, const float * w
     LinearEpilogue e;
     if (!linear_epilogue(e, bias, residual, res_dtype, ldr, out, out_dtype, ldo, act)) return IIAN_ERR_DTYPE;
     const bool whole = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t) x | (uintptr_t) w) % 16 == 0;
-    int tile = (form & 255) - 1, ks = form >> 8;
-    if (form == 0) ln_plan(N, M, K, whole, 148, &tile, &ks);
-    if (tile < 0 || ks < 1 || ks > 8) return IIAN_ERR_SHAPE;
+    const int groups = form == 0 ? ln_groups(M, K) : form >> 8, tile = form == 0 ? ln_plan(N, M, K, groups, 148) : (form & 255) - 1;
+    if (tile < 0 || tile > 4 || groups < 1 || groups > 8 || groups * 4 % LN_TILES[tile].warps != 0) return IIAN_ERR_SHAPE;
+    const int ks = groups * 4 / LN_TILES[tile].warps;
     return whole ? ln_go<4>(tile, x, ldx, w, N, M, K, ks, e, stream) : ln_go<1>(tile, x, ldx, w, N, M, K, ks, e, stream);
 }
