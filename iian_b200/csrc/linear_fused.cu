@@ -740,13 +740,14 @@ static double lf_estimate(int T, int N, int K, int sms, bool pair, bool swap, in
     const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8, x_cols = (T + 15) / 16 * 16;
     const double tiles = (swap ? 1.0 : (double) ((T + rows - 1) / rows)) * ((N + bn - 1) / bn), ctas = tiles * ks * group;
     int slots = sms / (group * ks) * (group * ks);
-    if (ks > 4) slots = std::min(slots, sms - sms / 9);          // clusters of six or eight leave some SMs of a GPC over
+    if (ks >= 4) slots = std::min(slots, sms - sms / (ks > 4 ? 9 : 12));          // clusters of four to eight leave some SMs of a GPC over
     const double waves = (double) (long long) ((ctas + slots - 1) / slots), active = std::min(ctas, (double) slots);
     const int kb = ((K + TC_BK - 1) / TC_BK + ks - 1) / ks, per = ((bn / 4 + ks - 1) / ks) | 1;
     if (swap) {
         const double block = std::max((bn + x_cols) * 128.0 * active / 12.2e6, std::max(0.217, x_cols * 2 / 1850.0 * 1.96));
-        const double t = std::max(waves * kb * block, 2.0 * K * ((double) N + T) / 5.28e6);
-        return t + (ks == 1 ? 0.17 + 0.86 * T / 128.0 : 1.31 + waves * 6.59 * ks * x_cols * per * 16 / 131072.0);
+        const double work = waves * kb * block, memory = 2.0 * K * ((double) N + T) / 5.28e6;    // the shorter one is not hidden as a whole
+        const double t = std::max(work, memory) + 0.25 * std::min(work, memory);
+        return t + (ks == 1 ? 0.17 + 0.86 * T / 128.0 : 1.31 + waves * 4.0 * ks * x_cols * per * 16 / 131072.0);
     }
     const double fill = (a_rows + (pair ? bn / 2 : bn)) * 128.0 / std::min(131.5e3, 17.8e6 / active);
     const double t = std::max(waves * kb * std::max(fill, std::max(0.253, bn * 2 / 1850.0 * 1.5)), 2.0 * K * ((double) N + T) / 3.32e6);
