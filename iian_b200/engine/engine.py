@@ -339,22 +339,21 @@ class Engine:
                         break
                     mgr.release_passed(rc, done)
                     if not mgr.allocate(rc, done, n):
-                        # those behind it give their pages back and begin again later; alone it cannot go on
-                        if k == 0 and len(live) == 1:
-                            raise RuntimeError(f"score: a sequence of {len(seqs[i])} tokens does not fit in the KV cache")
+                        # those behind it give their pages back and begin again later; where that is not enough it cannot go on
                         for j, c, _ in reversed(live[max(k, 1):]):
                             mgr.free(c)
                             out[j] = []
                             waiting.insert(0, j)
                         del live[max(k, 1):]
-                        break
+                        if k > 0:
+                            break
+                        if not mgr.allocate(rc, done, n):
+                            raise RuntimeError(f"score: a sequence of {len(seqs[i])} tokens does not fit in the KV cache")
                     want = range(max(0, first[i] - 1 - done), n)
                     entries.append(StepEntry(rc, seqs[i][done: done + n], done, want))
                     targets.append([seqs[i][done + j + 1] for j in want])
                     moved.append((live[k], n))
                     left -= n
-                if not entries:
-                    continue                    # the oldest one has the pages to itself now
                 got = self.runner.score(entries, targets)
                 values = got[0].tolist() if got is not None else []
                 self.runner.check_device_status()

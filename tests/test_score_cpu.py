@@ -80,6 +80,22 @@ def test_sequences_that_do_not_fit_together_wait_for_one_another(qwen):
     eng.cache.check_invariants()
 
 
+def test_sequences_none_of_which_fits_beside_a_request(qwen):
+    _, model, _ = qwen
+    from iian_b200 import SamplingParams
+    with ops.use_kernels(sm.ScoredFakes()):
+        eng = engine(model, kv_cache_tokens=96, max_model_len=96, budget=16, seqs=4)
+        req = eng.submit(random_tokens(503, 60, 1), SamplingParams(temperature=0.0, max_tokens=4))
+        while not req.output_tokens:
+            eng.step()
+        for lists in ([random_tokens(503, 90, i) for i in range(3)], [random_tokens(503, 20, 5), random_tokens(503, 90, 6), random_tokens(503, 91, 7)]):
+            with pytest.raises(RuntimeError, match="does not fit"):
+                eng.score(lists)
+        while not req.is_finished:
+            eng.step()
+    eng.cache.check_invariants()
+
+
 def test_beside_requests_under_way(qwen):
     _, model, want = qwen
     prompt, tokens = random_tokens(503, 30, 1), random_tokens(503, 40, 2)
