@@ -186,7 +186,7 @@ class PlainMLP(FeedForward):
 
     def kernel_libraries(self):
         if self.fused:
-            return ("linear_fused", "gemm_simt")
+            return ("linear_fused", "linear_f32", "gemm_simt")
         return ("residual_ops", "gemm_simt")
 
     def forward(self, x, ctx, residual=None):
