@@ -138,7 +138,9 @@ _sigs_done = set()
 
 
 # Programmatic dependent launch (see csrc/common.cuh).  IIAN_PDL names the kernel libraries whose launches get the
-# attribute ("gemm_stream,attention_mma"; "1": all, "0": none).  Default: the streaming product alone.  Its CTAs fill
+# attribute ("gemm_stream,attention_mma"; "1": all, "0": none).  Default: the streaming product, and the
+# products with an epilogue and the grouped routing, whose set-up runs beside the end of the kernel before (a product alone 2 us less in a row of
+# calls).  The streaming product's CTAs fill
 # their ring of shared memory with weights while the kernel before drains, and they cannot crowd that kernel out (a CTA
 # takes nearly all of an SM's shared memory, so it only becomes resident where one has left): 3.10 -> 2.91 ms per decode
 # step at batch 1, 3.60 -> 3.31 at batch 8.  With the attribute on every kernel of the step the register-bound kernels
