@@ -112,6 +112,52 @@ def test_float32_rows_have_the_same_bits_in_any_batch(k, m):
             assert torch.equal(out, whole[first: first + n])
 
 
+def test_float32_rows_far_apart():
+    store = torch.empty(8 * 2 ** 28 + 64, device="cuda")             # the ninth row begins 8 GB on
+    x = store.as_strided((9, 64), (2 ** 28, 1))
+    x.copy_(torch.randn(9, 64, device="cuda"))
+    w, out = torch.randn(70, 64, device="cuda") * 0.05, torch.empty(9, 70, device="cuda")
+    K().linear_act(x, w, out)
+    y, ref = reference(x, w, None, "none", None)
+    assert ((out.double() - ref).abs() <= tolerance(x, w, y, ref, "none", F32, False)).all()
+
+
+@pytest.mark.parametrize("n,k,m", [(1, 4096, 155), (40, 1027, 300)])
+def test_float32_captured_and_on_another_stream(n, k, m):
+    x, w, b = torch.randn(n, k, device="cuda"), torch.randn(m, k, device="cuda") * 0.05, torch.randn(m, device="cuda")
+    out, r = torch.empty(n, m, device="cuda"), torch.randn(n, m, device="cuda")
+    want = torch.empty(n, m, device="cuda")
+    K().linear_act(x, w, want, bias=b, activation="gelu", residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K().linear_act(x, w, out, bias=b, activation="gelu", residual=r)
+    side.synchronize()
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K().linear_act(x, w, out, bias=b, activation="gelu", residual=r)
+        K().linear_act(x, w, r, residual=r)
+    x.mul_(0.5)
+    start = r.clone()
+    K().linear_act(x, w, want, bias=b, activation="gelu", residual=start)
+    second = start.clone()
+    K().linear_act(x, w, second, residual=second)
+    graph.replay()
+    assert torch.equal(out, want) and torch.equal(r, second)
+
+
+@pytest.mark.parametrize("n,k,m", [(2, 64, 40), (33, 1027, 70)])
+def test_float32_infinities_and_nan_stay_in_their_rows(n, k, m):
+    x, w = torch.randn(n, k, device="cuda"), torch.randn(m, k, device="cuda")
+    clean, out = torch.empty(n, m, device="cuda"), torch.empty(n, m, device="cuda")
+    K().linear_act(x, w, clean)
+    x[n - 1, k - 1], w[m - 1, 0] = float("nan"), float("inf")
+    K().linear_act(x, w, out)
+    assert torch.equal(out[: n - 1, : m - 1], clean[: n - 1, : m - 1])
+    assert out[n - 1].isnan().all() and not out[: n - 1, m - 1].isfinite().any()
+
+
 @pytest.mark.parametrize("dtype,wdtype,k", [(BF, F32, 64), (F32, BF, 64), (BF, BF, 71), (BF, BF, 4)])
 def test_what_the_tensor_cores_do_not_take(dtype, wdtype, k):
     check(33, k, 50, dtype, BF, "relu", True, True, wdtype=wdtype)
