@@ -178,13 +178,13 @@ template <int KIND> __device__ __forceinline__ void lf_put(const LinearEpilogue 
     }
 }
 
-template <bool PAIR, bool SWAP, int KIND>
+// KPS: blocks of K a stage (two on pairs of SMs, one or two otherwise)
+template <bool PAIR, bool SWAP, int KPS, int KIND>
 __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b, const LfArgs p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = (unsigned char *) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);
     constexpr bool SCORE = KIND == LF_SCORE;
-    constexpr int KPS = PAIR ? 2 : 1;     // blocks of K a stage
     constexpr int ROWS = PAIR ? 2 * TC_BM : TC_BM;
     __shared__ __align__(8) unsigned long long full_bar[LF_STAGES], empty_bar[LF_STAGES], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_base_s;
@@ -212,9 +212,12 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
             }
         } else {
             const unsigned bar = smem_addr(&full_bar[s]);
-            mbar_expect_tx_warp(bar, SWAP ? (p.bn + p.x_cols) * TC_BK * 2 : kb_bytes);
-            tma_load_2d_warp(to, &map_a, kb * TC_BK, ya, bar);
-            tma_load_2d_warp(to + a_bytes, &map_b, kb * TC_BK, yb, bar);
+            mbar_expect_tx_warp(bar, KPS * (SWAP ? (p.bn + p.x_cols) * TC_BK * 2 : kb_bytes));
+#pragma unroll
+            for (int j = 0; j < KPS; j++) {
+                tma_load_2d_warp(to + j * kb_bytes, &map_a, (kb * KPS + j) * TC_BK, ya, bar);
+                tma_load_2d_warp(to + j * kb_bytes + a_bytes, &map_b, (kb * KPS + j) * TC_BK, yb, bar);
+            }
         }
     };
 
@@ -648,7 +651,7 @@ static int lf_sms() {
 // T, N, bn, ks, status, epi or score as given; PAIR: tiles of 256 rows on pairs of SMs.
 template <bool PAIR, bool SWAP, int KIND>
 static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, int K, int sms, cudaStream_t stream) {
-    constexpr int KPS = PAIR ? 2 : 1, ROWS = PAIR ? 2 * TC_BM : TC_BM;
+    constexpr int ROWS = PAIR ? 2 * TC_BM : TC_BM;
     // All of it whatever the call needs: two CTAs of a cluster that each waited for the tensor memory of an SM's other CTA, those two in turn
     // waiting for their clusters, would never end, so no SM may hold two.
     constexpr int kRing = kLfRing, smem = kLfSmem, kRecvMost = 80 * 1024;
@@ -657,7 +660,6 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
     const int a_rows = SWAP ? (p.bn + 7) / 8 * 8 : PAIR || p.T >= TC_BM ? TC_BM : (p.T + 7) / 8 * 8, half = SWAP ? p.x_cols : PAIR ? p.bn / 2 : p.bn;
     p.a_bytes = a_rows * TC_BK * 2;
     p.kb_bytes = p.a_bytes + half * TC_BK * 2;
-    p.stage_bytes = KPS * p.kb_bytes;
     const int over = (TC_BM - a_rows) * TC_BK * 2;                     // the last stage's product reads 128 rows too
     int ring = kRing;
     if (p.ks > 1) {
@@ -671,8 +673,12 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
         if (!p.recv_shared) ring = (kRing - recv) / 1024 * 1024;
         p.recv_off = p.recv_shared ? 0 : ring;
     }
+    // two blocks of K a stage where four such stages fit and every share has two: a stage costs the warps that copy and multiply some 200 ns
+    // whatever its size (128 x 128 x 16,384 55 us with one block a stage)
+    const int blocks = (K + TC_BK - 1) / TC_BK, kps = PAIR || ((ring - over) / (2 * p.kb_bytes) >= 4 && blocks / 2 >= p.ks) ? 2 : 1;
+    p.stage_bytes = kps * p.kb_bytes;
     p.stages = std::min(LF_STAGES, (ring - over) / p.stage_bytes);
-    p.all_kb = ((K + TC_BK - 1) / TC_BK + KPS - 1) / KPS;
+    p.all_kb = (blocks + kps - 1) / kps;
     p.m_tiles = SWAP ? 1 : (p.T + ROWS - 1) / ROWS;
     const long long tiles = (long long) p.m_tiles * ((p.N + p.bn - 1) / p.bn);
     const int group = (PAIR ? 2 : 1) * p.ks;
@@ -681,17 +687,17 @@ static int lf_launch(LfArgs & p, const void * x, long long ldx, const void * w, 
     p.units = p.ks > 1 ? p.num_tiles : std::min(p.num_tiles, sms / group);
     const int acc_cols = ((SWAP ? p.x_cols : p.bn) + 31) & ~31, bufs = p.units < p.num_tiles ? 2 : 1;      // (a CTA with one tile needs no second buffer)
     p.accs = 1;
-    while (p.accs < (KIND == LF_SCORE ? 2 : 4) && 2 * p.accs * bufs * acc_cols <= 512 && 2 * p.accs <= p.all_kb / p.ks) p.accs *= 2;
+    while (p.accs < (KIND == LF_SCORE ? 2 : 4) && 2 * p.accs * bufs * acc_cols <= 512 && 2 * p.accs <= p.all_kb / p.ks * kps) p.accs *= 2;
     p.buf_cols = p.accs * acc_cols;
     p.tmem_cols = 32;
     while (p.tmem_cols < (unsigned) (bufs * p.buf_cols)) p.tmem_cols *= 2;
-    auto kernel = linear_fused_kernel<PAIR, SWAP, KIND>;
-    static bool configured[64] = {};
+    auto kernel = kps == 2 ? linear_fused_kernel<PAIR, SWAP, 2, KIND> : linear_fused_kernel<PAIR, SWAP, PAIR ? 2 : 1, KIND>;
+    static bool configured[2][64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !configured[dev])) {
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !configured[kps - 1][dev])) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+        if (e == cudaSuccess && dev >= 0 && dev < 64) configured[kps - 1][dev] = true;
     }
     if (e != cudaSuccess) return 1000 + (int) e;
     CUtensorMap ma, mb;
