@@ -739,8 +739,8 @@ static int lf_even(int n, int parts, int step) { return std::max(32, ((n + parts
 
 // The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants are fitted to 35 shapes from
 // 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024, each timed in every form (the form it takes is 2 % slower than the best one on average, 16 % at
-// most).  A K block costs the longest of its copies (of an SM, and of all together), its products, and the quarter of a microsecond that a
-// block's instructions and commit take; the operands come from memory; then come the epilogue of a tile and, where K is shared, the exchange
+// most).  A K block costs the longest of its copies (of an SM, and of all together), its products, and the fifth of a microsecond or so that a
+// stage's instructions and commit take (less with two blocks a stage: not told apart here, which chose no better); the operands come from memory; then come the epilogue of a tile and, where K is shared, the exchange
 // of the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
 static double lf_estimate(int T, int N, int K, int sms, bool pair, bool swap, int bn, int ks) {
     const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8, x_cols = (T + 15) / 16 * 16;
@@ -760,9 +760,9 @@ static double lf_estimate(int T, int N, int K, int sms, bool pair, bool swap, in
     return t + (ks == 1 ? 2.74 * bn / 256 : 1.48 + waves * 10.4 * ks * a_rows * per * 16 / 131072.0);
 }
 
-// Whether w's rows are the product's: up to 64 rows of x always (1 x 4,096 x 4,096 8.6 us, the other way 10.1; 61 x 4,096 x 12,288 21.6 and 23.5; a
+// Whether w's rows are the product's: up to 64 rows of x always (1 x 4,096 x 4,096 7.8 us, the other way 8.9; 61 x 4,096 x 12,288 21.2 and 22.6; a
 // row of x then costs 16 columns of a product where it cost 128 rows, and with them the power that bounds a long run of such calls), up to 128
-// where K is long enough to matter (128 x 4,096 x 4,096 13.7 and 14.5, but 100 x 4,096 x 1,024 7.3 and 6.3).
+// where K is long enough to matter (128 x 4,096 x 4,096 12.6 and 12.8, 96 x 2,048 x 8,192 11.8 and 12.0, but 100 x 4,096 x 1,024 7.3 and 6.1).
 static bool lf_swaps(int T, int K) { return T <= 64 || (T <= TC_BM && K >= 2048); }
 
 static void lf_plan(int T, int N, int K, int sms, bool out_f32, bool * pair, bool * swap, int * bn, int * ks) {
