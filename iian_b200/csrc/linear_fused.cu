@@ -14,8 +14,9 @@
 // may have fewer rows than the 128 that the product reads of shared memory; what lies behind the real ones only reaches rows of the
 // accumulator that nobody reads.
 //
-// Few tiles: the K blocks of a tile are shared by a cluster of `ks` CTAs.  Each leaves its part in its shared memory, and each adds up all
-// parts, in their order, for its share of the tile.
+// Few tiles: the K blocks of a tile are shared by a cluster of `ks` CTAs.  Each sends its part into the others' shared memory, and each adds up
+// all parts, in their order, for its share of the tile.  Nothing is sent before every CTA of the cluster has begun: on pairs the barrier at the
+// start says so, single CTAs arrive at one there and wait for it before they send, when the products are long done.
 //
 // The softmax's sums: a thread walks its row's columns with a running maximum and sum and leaves them per tile; a second kernel joins a
 // row's.  The maximum is the running one, so no exponential overflows; an empty sum has the maximum minus infinity.
@@ -244,6 +245,10 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
     __syncthreads();
     pdl_wait();                                   // set-up runs beside the end of the kernel before; nothing in memory is read or written until here
     if constexpr (PAIR) cluster_sync_all();       // the peer's barriers exist before anything arrives on them
+    else if (p.ks > 1) {
+        __syncwarp();
+        cluster_arrive();                         // this CTA has begun: waited for before the parts are sent, on every way there
+    }
     tc_fence_after();
     const unsigned tmem_base = tmem_base_s;
 
@@ -477,6 +482,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
     __syncwarp();
     if constexpr (!SCORE) {
         if (p.ks > 1) {
+            if constexpr (!PAIR) cluster_wait();              // every CTA of the cluster has begun: its shared memory may be written
             if (p.recv_shared) cluster_sync_all();            // every CTA's ring is done with
             const int m0 = unit % m_tiles * ROWS + (int) rank * TC_BM, n0 = unit / m_tiles * bn, rows = min(TC_BM, p.T - m0);
             const unsigned recv = smem_addr(smem) + (unsigned) p.recv_off;
