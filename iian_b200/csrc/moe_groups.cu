@@ -374,11 +374,17 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs 
         __syncwarp();
         mine_e = chosen[lane < p.top ? lane : 0];
     }
+    // The chosen scores again, a lane each, for the weights: with the digits that the order could do without (an __expf is off by a unit in the
+    // last place for every 0.85 of its argument), and a sigmoid in a form that does not overflow.  Scores of 32 bits end near e^-87: where a
+    // smaller one has to be divided by the sum of the chosen, the token is done in 64.
     float mine = 0.0f;
+    bool small = false;
     if (lane < p.top) {
-        const float x = p.logits[t * p.ld + mine_e];
-        mine = p.softmax ? __expf(x - mx) * most : route_sigmoid(x);
+        const float x = p.logits[t * p.ld + mine_e], d = p.softmax ? x - mx : x, e = expf(p.softmax ? d : -fabsf(x));
+        mine = p.softmax ? e * most : (x < 0.0f ? e : 1.0f) / (1.0f + e);
+        small = mine < 1e-36f && d > -750.0f;                // (below that 64 bits have nothing either)
     }
+    if (p.renorm && __any_sync(0xffffffffu, small)) unsure = true;
     if (unsure) {
         route_exact<SLOTS>(p, t);
         return;
