@@ -79,9 +79,18 @@ __device__ __forceinline__ float lf_exp2(float x) {
     return y;
 }
 __device__ __forceinline__ float lf_finite_or_zero(float m) { return fabsf(m) < CUDART_INF_F ? m : 0.0f; }
-// c tanh(z / c) with the hardware's exponential: tanh's absolute error is a few 1e-7
-__device__ __forceinline__ float lf_cap_fast(float z, float cap, float two_over_cap_log2e) {
-    return cap * (1.0f - __fdividef(2.0f, 1.0f + lf_exp2(z * two_over_cap_log2e)));
+// c tanh(z / c) within 2.2 units of 2^-22 of its value, for the sums and for the target's logit.  From |u| = 0.8 on, u = z / c, it is c (1 - 2 / (1 +
+// e^2u)) with the hardware's exponential, whose difference would lose the digits of small u (1e-4 at a cap of 1,000); below, z times a polynomial
+// in u^2 (minimax for tanh(u) / u, 4e-9).
+__device__ __forceinline__ float lf_capped(float z, float cap, float inv_cap) {
+    const float u = z * inv_cap, v = u * u, zv = z * v;
+    const float q = __fdividef(2.0f, 1.0f + lf_exp2(2.8853900817779268f * fabsf(u)));
+    float t = fmaf(v, 0.0015676724f, -0.007374115f);
+    t = fmaf(v, t, 0.02127475f);
+    t = fmaf(v, t, -0.053841557f);
+    t = fmaf(v, t, 0.13332023f);
+    t = fmaf(v, t, -0.3333328f);
+    return fabsf(u) < 0.8f ? fmaf(zv, t, z) : copysignf(cap * (1.0f - q), z);
 }
 
 // LF_COLS columns of 32 lanes
@@ -132,12 +141,12 @@ template <typename OP> __device__ __forceinline__ float lf_over_lanes(float (&v)
 }
 
 // 32 columns of a row, `live` of them in the matrix, into the row's running maximum and sum
-__device__ __forceinline__ void lf_take(const unsigned * r, int live, float cap, float two_over_cap_log2e, float & m, float & s) {
+__device__ __forceinline__ void lf_take(const unsigned * r, int live, float cap, float inv_cap, float & m, float & s) {
     float z[32], mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
     for (int i = 0; i < 32; i++) {
         z[i] = __uint_as_float(r[i]);
-        if (cap != 0.0f) z[i] = lf_cap_fast(z[i], cap, two_over_cap_log2e);
+        if (cap != 0.0f) z[i] = lf_capped(z[i], cap, inv_cap);
         if (i >= live) z[i] = -CUDART_INF_F;
         mx[i & 3] = fmaxf(mx[i & 3], z[i]);
     }
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
     } else if (warp >= 2) {
         // ---- epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 -----------------------------------
         const int q = warp & 3, half_w = (warp - 2) >> 2;          // the second four warps take every other columns
-        const float cap_factor = SCORE && p.score.cap != 0.0f ? 2.0f * kLog2e / p.score.cap : 0.0f;
+        const float inv_cap = SCORE && p.score.cap != 0.0f ? 1.0f / p.score.cap : 0.0f;
         int use = 0;
         for (int tile = unit; tile < num_tiles; tile += units, use++) {
             const int buf = use & 1;
@@ -355,7 +364,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
                             z[i] = __uint_as_float(r[i]);
-                            if (p.score.cap != 0.0f) z[i] = lf_cap_fast(z[i], p.score.cap, cap_factor);
+                            if (p.score.cap != 0.0f) z[i] = lf_capped(z[i], p.score.cap, inv_cap);
                             if (lane >= limit) z[i] = -CUDART_INF_F;
                             v[i] = z[i];
                         }
@@ -370,7 +379,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
                         while (here != 0) {                               // (a target among this warp's rows of w)
                             const int c = __ffs(here) - 1, from = __shfl_sync(0xffffffffu, rel, c);
                             const float x = __uint_as_float(lf_pick(r, c));
-                            if (lane == from) p.score.lp[c0 + c] = p.score.cap != 0.0f ? p.score.cap * tanhf(x / p.score.cap) : x;
+                            if (lane == from) p.score.lp[c0 + c] = p.score.cap != 0.0f ? lf_capped(x, p.score.cap, inv_cap) : x;
                             here &= here - 1;
                         }
                     }
@@ -418,10 +427,10 @@ __global__ void __launch_bounds__(LF_THREADS, 1) linear_fused_kernel(const __gri
 #pragma unroll
                             for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
                         }
-                        lf_take(r, cols - c0, p.score.cap, cap_factor, m, s);
+                        lf_take(r, cols - c0, p.score.cap, inv_cap, m, s);
                         if (target >= c0 && target < c0 + 32 && target < cols) {
                             const float z = __uint_as_float(lf_pick(r, target - c0));
-                            p.score.lp[row] = p.score.cap != 0.0f ? p.score.cap * tanhf(z / p.score.cap) : z;
+                            p.score.lp[row] = p.score.cap != 0.0f ? lf_capped(z, p.score.cap, inv_cap) : z;
                         }
                     }
                     if (row < p.T) p.score.part[((size_t) n_tile * 2 + half_w) * p.T + row] = make_float2(m, s);
