@@ -208,10 +208,15 @@ class Model:
         for idx, call in enumerate(order):
             select = ctx.out_rows if idx == len(order) - 1 else None
             block = self.blocks[call.layer]
+            # what the stream's last writer left of it in the activation dtype is true until the next one has run, whether that one
+            # took it or not
+            copy = ctx.step_cache.get("stream_act")
             if call.before is not None:
                 part = self.stream_parts[call.before]
                 turn = {"turn": call.turn} if getattr(part, "wants_turn", False) else {}
                 residual, delta = part.forward(residual, delta, ctx, **turn)
+                if copy is not None and ctx.step_cache.get("stream_act") is copy:
+                    del ctx.step_cache["stream_act"]
             extra = {}
             if idx + 1 < len(order) and getattr(block, "accepts_next_norm", False):
                 # the block after this one: its first norm may ride in this block's last product
@@ -219,6 +224,8 @@ class Model:
                 if getattr(nxt, "accepts_next_norm", False):
                     extra = {"next_norm": nxt.mixer_norm, "next_consumer": nxt.mixer}
             residual, delta = block.forward(residual, delta, ctx, storage.view(call.cache), call.writes_cache, select, **extra)
+            if copy is not None and ctx.step_cache.get("stream_act") is copy:
+                del ctx.step_cache["stream_act"]
         if not order:
             from .. import ops
             sel = ctx.buf("residual_rows", (ctx.out_rows.shape[0], residual.shape[1]), residual.dtype)

@@ -82,7 +82,7 @@ class Identity(Norm):
 
     What is still owed to the stream (a tensor or a ``NormedAddend``) is added first, as every norm does, and the stream's copy in
     the activation dtype leaves the same kernel.  Whoever wrote the stream last may have left that copy already
-    (``ctx.step_cache["stream_act"]``); in 32-bit the stream is its own copy."""
+    (``ctx.step_cache["stream_act"]``, which the model drops behind whatever runs next); in 32-bit the stream is its own copy."""
 
     def kernel_libraries(self):
         return ("residual_ops",)
