@@ -223,6 +223,13 @@ static int ln_go(int tile, const float * x, long long ldx, const float * w, int 
 
 using namespace iian;
 
+// The form of a product with M of a matrix's `of` rows that gives the bits which the product with all of them does.
+IIAN_API int iian_linear_act_f32_form(int N, int M, int of, int K) {
+    if (N <= 0 || M <= 0 || of < M || K <= 0) return 0;
+    const int groups = ln_groups(of, K);
+    return ln_plan(N, M, K, groups, 148) + 1 | groups << 8;
+}
+
 // x rows ldx apart; form 0: the tile and the groups of warps that suit the sizes, else tile + 1 | groups << 8
 IIAN_API int iian_linear_act_f32(const float * x, long long ldx, const float * w, const float * bias, const void * residual, int res_dtype,
                                  long long ldr, void * out, int out_dtype, long long ldo, int N, int M, int K, int act, int form, cudaStream_t stream) {

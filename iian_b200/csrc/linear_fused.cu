@@ -577,18 +577,18 @@ __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __res
     const long long row = (long long) blockIdx.x * rows + r;
     float m = -CUDART_INF_F, s = 0.0f;
     auto add = [&](float m2, float s2) {
-        const float m1 = fmaxf(m, m2), ref = lf_finite_or_zero(m1) * kLog2e;
-        s = (s == 0.0f ? 0.0f : s * lf_exp2(fmaf(m, kLog2e, -ref))) + (s2 == 0.0f ? 0.0f : s2 * lf_exp2(fmaf(m2, kLog2e, -ref)));
+        const float m1 = fmaxf(m, m2), ref = lf_finite_or_zero(m1);
+        s = (s == 0.0f ? 0.0f : s * lf_exp2((m - ref) * kLog2e)) + (s2 == 0.0f ? 0.0f : s2 * lf_exp2((m2 - ref) * kLog2e));
         m = m1;
     };
     if (row < T) {
 #pragma unroll 8
         for (int i = seg; i < n_tiles; i += segs) m = fmaxf(m, part[(size_t) i * T + row].x);
-        const float ref = lf_finite_or_zero(m) * kLog2e;
+        const float ref = lf_finite_or_zero(m);              // (differences first: where the maximum is one part's its factor is 1 exactly)
 #pragma unroll 8
         for (int i = seg; i < n_tiles; i += segs) {
             const float2 v = part[(size_t) i * T + row];
-            s += v.y == 0.0f ? 0.0f : v.y * lf_exp2(fmaf(v.x, kLog2e, -ref));
+            s += v.y == 0.0f ? 0.0f : v.y * lf_exp2((v.x - ref) * kLog2e);
         }
     }
     sm[threadIdx.x] = m;
@@ -609,14 +609,15 @@ __global__ void __launch_bounds__(512) logprobs_join_kernel(const float2 * __res
     }
 }
 
-// Columns v0 .. v0 + P of the logits of T rows, as they lie in memory, into the rows' maxima and sums: part `split` of gridDim.y of a piece
-// whose parts begin at part[first].  For element types and sizes that the tensor cores' product does not take.
+// Columns v0 .. v0 + P of the logits of T rows, as they lie in memory, into the rows' maxima and sums: a part for every `columns` of them, from
+// part[first] on.  For element types and sizes that the tensor cores' product does not take.  Where a part begins and ends goes by the
+// vocabulary alone, so that a row's sum has the same bits whatever rows are beside it.
 __global__ void __launch_bounds__(256) logprobs_piece_kernel(const float * __restrict__ logits, int T, int P, int v0, const int * __restrict__ targets,
-                                                             float * __restrict__ lp, float2 * __restrict__ part, int first, float cap) {
+                                                             float * __restrict__ lp, float2 * __restrict__ part, int first, int columns, float cap) {
     __shared__ float sm[8], ss[8];
     pdl_wait();
     const size_t row = blockIdx.x;
-    const int splits = gridDim.y, c0 = (int) ((long long) P * blockIdx.y / splits), c1 = (int) ((long long) P * (blockIdx.y + 1) / splits);
+    const int c0 = (int) blockIdx.y * columns, c1 = min(P, c0 + columns);
     const float * z = logits + row * P;
     float m = -CUDART_INF_F, s = 0.0f;
     auto add = [&](float m2, float s2) {
@@ -890,13 +891,14 @@ IIAN_API int iian_linear_logprobs(const void * x, long long ldx, const void * w,
     return lf_join(part, (swap ? 4 : 2) * ((N + p.bn - 1) / p.bn), T, N, targets, lp, lse, stream);
 }
 
-// The same from logits in memory, a piece of the vocabulary at a time: logits [T, P] float32 hold columns v0 .. v0 + P, whose `splits` parts
-// become part[first ..] (the last piece's call is followed by one of iian_linear_logprobs_join over all parts).
+// The same from logits in memory, a piece of the vocabulary at a time: logits [T, P] float32 hold columns v0 .. v0 + P; every `columns` of them
+// become one of part[first ..] (the last piece's call is followed by one of iian_linear_logprobs_join over all parts).
 IIAN_API int iian_linear_logprobs_piece(const float * logits, int T, int P, int v0, const int * targets, float * lp, float * part, int first,
-                                        int splits, float cap, cudaStream_t stream) {
+                                        int columns, float cap, cudaStream_t stream) {
     if (T <= 0 || P <= 0) return IIAN_OK;
-    if (splits <= 0 || splits > 65535 || first < 0 || cap < 0.0f) return IIAN_ERR_SHAPE;
-    return iian_launch(logprobs_piece_kernel, dim3((unsigned) T, (unsigned) splits), dim3(256), 0, stream, logits, T, P, v0, targets, lp, (float2 *) part, first, cap);
+    if (columns <= 0 || P > 2147483647 - columns || (P + columns - 1) / columns > 65535 || first < 0 || cap < 0.0f) return IIAN_ERR_SHAPE;
+    return iian_launch(logprobs_piece_kernel, dim3((unsigned) T, (unsigned) ((P + columns - 1) / columns)), dim3(256), 0, stream, logits, T, P, v0, targets, lp,
+                       (float2 *) part, first, columns, cap);
 }
 IIAN_API int iian_linear_logprobs_join(const float * part, int parts, int T, int V, const int * targets, float * lp, float * lse, cudaStream_t stream) {
     if (T <= 0) return IIAN_OK;

@@ -181,6 +181,7 @@ _LINEAR_ACT_ARGS = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c
                     c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
 _GEMM_SIMT_ARGS = [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
 _LINEAR_ACT_F32_ARGS = _LINEAR_ACT_ARGS[:-2] + [c_void_p]
+_LINEAR_ACT_F32_FORM_ARGS = [c_int, c_int, c_int, c_int]
 _LINEAR_ACT_SIMT_ARGS = [c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong,
                          c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p]
 _LINEAR_LOGPROBS_TILES_ARGS = [c_int, c_int, c_int]
@@ -2421,6 +2422,7 @@ class CudaKernels:
         _check(fn(xp, _CODE[x.dtype], ldx, wp, _CODE[w.dtype], bp, rp, rc, ldr, op, oc, ldo, n, m, k, act, stream), "linear_act_simt")
 
     SCORE_ROWS = 16384          # rows of one launch: their partial sums take up to 8 bytes a row and 128 columns
+    SCORE_COLUMNS = 2048        # columns of a partial sum of theirs
     SCORE_PIECE = 1 << 24       # logits that are in memory at a time where the tensor cores' product does not take the operands
 
     def linear_logprobs(self, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, logprobs: torch.Tensor, lse: torch.Tensor,
@@ -2430,7 +2432,10 @@ class CudaKernels:
 
         x [N, K] (rows may be apart) and w [V, K] float32 or bfloat16, targets int32 [N].  A negative target is none: its log-probability is
         0; one of V or more gives what is no number.  A row of nothing but minus infinity has the log-sum-exp minus infinity.  The working
-        memory, a pair of floats a row and some 200 columns, is the call's own."""
+        memory is the call's own: a pair of floats a row and some 200 columns, and where x and w are not both bfloat16 with rows of whole 16-byte
+        pieces the logits of a piece of the vocabulary.  Of float32 operands, and of mixed ones, a row has the same bits whatever rows are
+        beside it; of bfloat16 ones the sums' order goes by the number of rows, and the tensor cores cut off what they add up (2^-23 of the
+        sum for each 16 of K)."""
         n, k, v, xp, ldx, wp, tc = self._product_rows(x, w, "linear_logprobs")
         if targets.shape != (n,) or logprobs.shape != (n,) or lse.shape != (n,) or v < 1:
             raise KernelError(f"linear_logprobs: x {tuple(x.shape)}, w {tuple(w.shape)}; targets, logprobs and lse [N] do not fit")
@@ -2458,33 +2463,39 @@ class CudaKernels:
             self._logprobs_pieces(x[r: r + t], xp + r * ldx * esize, ldx, w, wp, at, t, v, k, cap, stream)
 
     def _logprobs_pieces(self, x, xp, ldx, w, wp, at, t, v, k, cap, stream) -> None:
-        """The same with the logits of a piece of the vocabulary at a time in memory, from the product that takes every type and size."""
-        width = min(v, max(4096, self.SCORE_PIECE // t))
-        splits = max(1, min(64, width // 2048, 1024 // t))
-        pieces = -(-v // width)
-        logits = torch.empty(t * width, dtype=torch.float32, device=x.device)
-        part = torch.empty(2 * pieces * splits * t, dtype=torch.float32, device=x.device)
+        """The same with the logits of a piece of the vocabulary at a time in memory, from the products that take every type and size."""
+        columns = self.SCORE_COLUMNS
+        width = min(v, max(4096, self.SCORE_PIECE // t) // columns * columns)
+        parts = -(-v // columns)
         f32 = x.dtype == w.dtype == torch.float32
-        many = f32 and t >= 128 and ldx == k and k % 4 == 0          # the plain product's large tiles (1,470 rows of 14,284 x 1,072: 1,000 us, the other's 1,280)
-        if many:
+        # Which product it is goes by what w is and never by the rows: the plain one, whose every form adds up in one order, and for rows of w that
+        # do not begin on 16 bytes the one with an epilogue, whose order is that of K and the vocabulary.
+        plain = f32 and k % 4 == 0 and wp % 16 == 0
+        if plain and (ldx != k or xp % 16):
+            x = x.clone(memory_format=torch.contiguous_format)
+            xp = x.data_ptr()
+        logits = torch.empty(t * width, dtype=torch.float32, device=x.device)
+        part = torch.empty(2 * parts * t, dtype=torch.float32, device=x.device)
+        if plain:
             product = _entry("gemm_simt", "iian_gemm_simt", _GEMM_SIMT_ARGS)
         elif f32:
             product = _entry("linear_f32", "iian_linear_act_f32", _LINEAR_ACT_F32_ARGS)
+            form_of = _entry("linear_f32", "iian_linear_act_f32_form", _LINEAR_ACT_F32_FORM_ARGS)
         else:
             product = _entry("gemm_simt", "iian_linear_act_simt", _LINEAR_ACT_SIMT_ARGS)
         take = _entry("linear_fused", "iian_linear_logprobs_piece", _LINEAR_LOGPROBS_PIECE_ARGS)
-        for i in range(pieces):
-            v0, p = i * width, min(width, v - i * width)
+        for v0 in range(0, v, width):
+            p = min(width, v - v0)
             piece = wp + v0 * k * w.element_size()
-            if many:
+            if plain:
                 _check(product(xp, F32, piece, F32, logits.data_ptr(), F32, t, p, k, stream), "gemm_simt")
             elif f32:
-                _check(product(xp, ldx, piece, 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k, 0, 0, stream), "linear_act_f32")
+                _check(product(xp, ldx, piece, 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k, 0, form_of(t, p, v, k), stream), "linear_act_f32")
             else:
                 _check(product(xp, _CODE[x.dtype], ldx, piece, _CODE[w.dtype], 0, 0, 0, 0, logits.data_ptr(), F32, p, t, p, k, 0, stream), "linear_act_simt")
-            _check(take(logits.data_ptr(), t, p, v0, at[0], at[1], part.data_ptr(), i * splits, splits, cap, stream), "linear_logprobs_piece")
+            _check(take(logits.data_ptr(), t, p, v0, at[0], at[1], part.data_ptr(), v0 // columns, columns, cap, stream), "linear_logprobs_piece")
         join = _entry("linear_fused", "iian_linear_logprobs_join", _LINEAR_LOGPROBS_JOIN_ARGS)
-        _check(join(part.data_ptr(), pieces * splits, t, v, *at, stream), "linear_logprobs_join")
+        _check(join(part.data_ptr(), parts, t, v, *at, stream), "linear_logprobs_join")
 
     # ---- sampling ------------------------------------------------------------------------
     def argmax(self, logits: torch.Tensor, out: torch.Tensor) -> None:
