@@ -110,7 +110,8 @@ class LMHead(Head):
         self.weight = table
 
     def kernel_libraries(self):
-        return ("gemm_simt",) + (("residual_ops",) if self.softcap is not None else ())
+        # (the last two are the score's: the first scored prompt of a running server waits for no compiler)
+        return ("gemm_simt",) + (("residual_ops",) if self.softcap is not None else ()) + ("linear_fused", "linear_f32")
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         logits = ctx.buf("logits", (x.shape[0], self.vocab), torch.float32)
