@@ -79,6 +79,7 @@ def _stream() -> int:
 
 
 _entries = {}
+_SIZE_MOST = 0x7fffffff        # a size that is one of the entry points' ints (a larger one would arrive there as another number)
 
 
 def _entry(lib_name: str, fn_name: str, argtypes):
@@ -1408,6 +1409,8 @@ class CudaKernels:
     def moe_route(self, logits: torch.Tensor, top: int, ids: torch.Tensor, weights: torch.Tensor) -> None:
         """Router logits (float32, may be a column slice) -> the ``top`` experts of each token by sigmoid score, and the scores."""
         n, e = logits.shape
+        if n > _SIZE_MOST:
+            raise KernelError("moe_route_grouped: sizes go up to 2,147,483,647")
         if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top):
             raise KernelError("moe_route: logits float32 [N, E]; ids / weights [N, top]")
         lp, ld = self._rows(logits, "router logits")
@@ -2165,6 +2168,8 @@ class CudaKernels:
         """Router logits (float32, may be a column slice) plus ``bias`` -> the ``top`` experts with the largest values (ties to
         the lower index) and the softmax over those values alone."""
         n, e = logits.shape
+        if n > _SIZE_MOST:
+            raise KernelError("moe_route_grouped: sizes go up to 2,147,483,647")
         if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top) or (bias is not None and bias.numel() != e):
             raise KernelError("moe_route_softmax: logits float32 [N, E]; bias [E]; ids / weights [N, top]")
         lp, ld = self._rows(logits, "router logits")
@@ -2177,6 +2182,8 @@ class CudaKernels:
         """Scores ``s = softmax(logits)`` (float32, may be a column slice); the ``top`` outputs with the largest ``s + correction``
         (ties to the lower index), each weighing ``scale * s``."""
         n, e = logits.shape
+        if n > _SIZE_MOST:
+            raise KernelError("moe_route_grouped: sizes go up to 2,147,483,647")
         if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top) \
                 or (correction is not None and correction.numel() != e):
             raise KernelError("moe_route_corrected: logits float32 [N, E]; correction [E]; ids / weights [N, top]")
@@ -2344,6 +2351,8 @@ class CudaKernels:
         if logits.dim() != 2:
             raise KernelError("moe_route_grouped: logits float32 [N, E]")
         n, e = logits.shape
+        if n > _SIZE_MOST:
+            raise KernelError("moe_route_grouped: sizes go up to 2,147,483,647")
         if logits.dtype != torch.float32 or ids.shape != (n, top) or weights.shape != (n, top) or (correction is not None and correction.numel() != e):
             raise KernelError("moe_route_grouped: logits float32 [N, E]; correction [E]; ids / weights [N, top]")
         if score != "sigmoid" and score != "softmax":
@@ -2372,6 +2381,8 @@ class CudaKernels:
         if x.dtype not in _CODE or w.dtype not in _CODE:
             raise KernelError(f"{what}: x and w are float32 or bfloat16")
         n, k = xs
+        if k > _SIZE_MOST or ws[0] > _SIZE_MOST:
+            raise KernelError(f"{what}: sizes go up to 2,147,483,647")
         xp, ld = _row_place(x, what)
         if n <= 1:
             ld = k
@@ -2389,6 +2400,8 @@ class CudaKernels:
         other than that out overlaps none of them.  ``activation``: ``none``, ``silu``, ``gelu_tanh``, ``gelu`` (by erf), ``relu``, ``relu2``.  ``form``: a
         tile other than the one that is chosen (csrc/linear_fused.cu, linear_f32.cu)."""
         n, k, m, xp, ldx, wp, tc = self._product_rows(x, w, "linear_act")
+        if n > _SIZE_MOST:
+            raise KernelError("linear_act: sizes go up to 2,147,483,647")
         act = self.LINEAR_ACTIVATIONS.get(activation)
         if act is None:
             raise KernelError(f"linear_act: activation {activation!r} has no kernel ({', '.join(self.LINEAR_ACTIVATIONS)})")
