@@ -2440,7 +2440,7 @@ class CudaKernels:
 
     def linear_logprobs(self, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, logprobs: torch.Tensor, lse: torch.Tensor,
                         softcap: Optional[float] = None, form: int = 0) -> None:
-        """Log-probabilities of given tokens without the logits: with ``z = x w^T`` (and ``z = c tanh(z / c)`` where ``softcap`` is c),
+        """Log-probabilities of given tokens without the logits: with ``z = x w^T`` (and ``z = c tanh(z / c)`` where ``softcap`` is c, 2^-126 to 3e38),
         ``lse[t] = log sum_v exp z[t, v]`` and ``logprobs[t] = z[t, targets[t]] - lse[t]``, all float32.
 
         x [N, K] (rows may be apart) and w [V, K] float32 or bfloat16, targets int32 [N].  A negative target is none: its log-probability is
@@ -2453,8 +2453,8 @@ class CudaKernels:
         if targets.shape != (n,) or logprobs.shape != (n,) or lse.shape != (n,) or v < 1:
             raise KernelError(f"linear_logprobs: x {tuple(x.shape)}, w {tuple(w.shape)}; targets, logprobs and lse [N] do not fit")
         cap = float(softcap) if softcap is not None else 0.0
-        if not 0.0 <= cap < float("inf") or (softcap is not None and cap == 0.0):
-            raise KernelError("linear_logprobs: softcap must be positive")
+        if softcap is not None and not 2.0 ** -126 <= cap <= 3e38:
+            raise KernelError(f"linear_logprobs: softcap must be positive, between 2^-126 and 3e38 (got {cap})")
         tp, op = _whole(targets, "linear_logprobs targets", torch.int32), _whole(logprobs, "linear_logprobs out", torch.float32)
         sp = _whole(lse, "linear_logprobs lse", torch.float32)
         if op == sp and n > 0:

@@ -70,3 +70,9 @@ def test_both_ways_say_the_same():
         got.append(lp)
     # each by the bound above: K = 64, sum |x w| below 20, logits below 6
     assert (got[0] - got[1]).abs().max().item() <= 2 * (20 * 10 * 2.0 ** -23 + 64 * 20 * 2.0 ** -24 / 2 + 64 * 2.0 ** -24 * 12 + 300 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("cap", [2.0 ** -126, 3e38])
+@pytest.mark.parametrize("dtype,n,k", [(BF, 3, 64), (BF, 150, 64), (F32, 9, 64), (BF, 9, 67)])
+def test_the_least_and_the_largest_cap(dtype, n, k, cap):
+    check(n, k, 503, cap, dtype)

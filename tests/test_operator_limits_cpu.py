@@ -1,4 +1,5 @@
-"""What the kernel layer refuses before it looks for a device: sizes that no 32-bit number holds (of tensors that no memory holds either)."""
+"""What the kernel layer refuses before it looks for a device: sizes that no 32-bit number holds (of tensors that no memory holds either), caps that
+are none in 32 bits."""
 import pytest
 import torch
 
@@ -29,3 +30,15 @@ def test_scores(k, v):
 def test_routing(n, e):
     with pytest.raises(KernelError, match="2,147,483,647"):
         CudaKernels().moe_route_grouped(t(n, e, dtype=F32), 1, t(n, 1, dtype=I32), t(n, 1, dtype=F32))
+
+
+@pytest.mark.parametrize("cap", [1e39, 1e300, 1e-46, 1e-40, 5e-324])
+def test_caps_that_32_bits_do_not_hold(cap):
+    with pytest.raises(KernelError, match="softcap"):
+        CudaKernels().linear_logprobs(t(2, 8), t(4, 8), t(2, dtype=I32), t(2, dtype=F32), t(2, dtype=F32), softcap=cap)
+
+
+@pytest.mark.parametrize("cap", [2.0 ** -126, 30, 30.0, 3e38, None])
+def test_caps_that_they_do(cap):
+    with pytest.raises(KernelError, match="two tensors"):           # (the next thing that is looked at)
+        CudaKernels().linear_logprobs(t(2, 8), t(4, 8), t(2, dtype=I32), t(2, dtype=F32), t(2, dtype=F32), softcap=cap)
