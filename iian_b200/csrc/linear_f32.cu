@@ -6,10 +6,12 @@
 // waits for.  The warps' parts are added at the end, in their order, through shared memory and the cluster's.  So a thread has up to 8 x 8
 // sums although a CTA's tile is small enough for every SM to have some, and reads 16 bytes of shared memory per 16 multiply-adds.  What part
 // of K a warp has depends on K and on the rows of w: a row of x has the same bits whatever rows are beside it.
-// What bounds it: many rows, the packed multiply-adds, of which an SM takes some 60 % of what the pipe's width says, whatever feeds them (301 x
-// 2,048 x 1,024 48 us, of which 17.5 at the full width; the plain product's form with tiles that every warp shares 54); few rows, the
-// weights (1 x 12,288 x 4,096 45 us, 4.4 TB/s); few of everything, the latency of a ring's first turn and the join (1 x 155 x 9,596 14 us, one
-// chain over K 49).
+// What bounds it: many rows, the main loop, which takes 55 % of the multiply-adds that the pipe's width says (a 24 x 64 tile 11.3 us per 1,024 of
+// K; the plain product's 64 x 128 tile, which reads shared memory half as often for a multiply-add, has 78 %), and the tiles' ends, 1.6 us each in
+// which an SM's half multiplies nothing: 301 x 2,048 x 1,024 49 us, of which 17.5 at the full width and some 9 the ends of its six tiles an SM (832
+// CTAs over 296 places; the multiply-add pipe is busy for 44 % of the time); the plain product's form with tiles that every warp shares 54.  Few
+// rows, the weights (1 x 12,288 x 4,096 45 us, 4.4 TB/s); few of everything, the latency of a ring's first turn and the join (1 x 155 x 9,596
+// 14 us, one chain over K 49).
 // Each sum is a pair, of the even k and of the odd ones, so that packed multiply-adds take the operands as they lie in memory; a chain then is
 // K over twice the warps long, and rounds less than one over all of K.
 // Lanes are dealt so that neighbours share a row of one operand or of the other (bits 0 and 4 pick the row of x, bits 1 to 3 that of w).

@@ -65,7 +65,8 @@ struct LfArgs {
     int per, inv_per, recv_off, recv_ld, recv_rows, recv_shared;
     // a tile's K blocks go to `accs` accumulators in turn, added up in the epilogue: the sums in tensor memory are not rounded but cut off, so
     // that the error grows with the length of the chain, and products into one accumulator wait for one another (90 ns each however few
-    // columns they have); buf_cols: columns of all of them
+    // columns they have); buf_cols: columns of all of them.  Tiles of 256 columns leave room for one (2,048 x 12,288 x 4,096 in bfloat16 differs
+    // from sums in float32 by 1.6e-4 of its norm, a tenth of what the rounding of the outputs does, and 2,048 scores by 6e-7)
     int accs, buf_cols;
     unsigned tmem_cols;
     TcStatus * status;
@@ -753,11 +754,12 @@ static int lf_check(int T, int N, int K, const void * x, long long ldx, const vo
 
 static int lf_even(int n, int parts, int step) { return std::max(32, ((n + parts - 1) / parts + step - 1) / step * step); }
 
-// The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants are fitted to 35 shapes from
-// 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024, each timed in every form (the form it takes is 2 % slower than the best one on average, 16 % at
-// most).  A K block costs the longest of its copies (of an SM, and of all together), its products, and the fifth of a microsecond or so that a
-// stage's instructions and commit take (less with two blocks a stage: not told apart here, which chose no better); the operands come from memory; then come the epilogue of a tile and, where K is shared, the exchange
-// of the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
+// The tile and the shares of K that a call of these sizes takes: the least of an estimate in us, whose constants were fitted to 35 shapes from
+// 1 x 4,096 x 1,024 to 4,096 x 1,024 x 1,024 with one block of K a stage.  Timed in every form as the stages are now, the form it takes is 2.3 %
+// slower than the best one on average, and 17 % at most (256 x 4,096 x 12,288: 39.8 us, 34.1).  A K block costs the longest of its copies
+// (of an SM, and of all together), its products, and the fifth of a microsecond or so that a stage's instructions and commit take (less with two
+// blocks a stage: an estimate told of that chose worse); the operands come from memory; then come the epilogue of a tile and, where K is shared,
+// the exchange of the parts.  Sums in float32 over a long K stay with tiles of 128 columns, which leave room for two accumulators.
 static double lf_estimate(int T, int N, int K, int sms, bool pair, bool swap, int bn, int ks) {
     const int rows = pair ? 256 : 128, group = pair ? 2 : 1, a_rows = pair || T >= 128 ? 128 : (T + 7) / 8 * 8, x_cols = (T + 15) / 16 * 16;
     const double tiles = (swap ? 1.0 : (double) ((T + rows - 1) / rows)) * ((N + bn - 1) / bn), ctas = tiles * ks * group;

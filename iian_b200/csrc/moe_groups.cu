@@ -10,9 +10,10 @@
 // than these can tell, does its token again in 64.  A score that is no number is the smallest; a row whose chosen scores are all 0
 // weighs 0 (a softmax over logits of minus infinity alone is such a row).
 //
-// What bounds it: the integer pipe, that is the chain of `top` reductions and the groups' ranks, and the latency of the tokens that need 64
-// bits.  Sigmoid scores with a correction, 8 of 256 experts in 8 groups: 61 tokens 3.4 us (2.3 of them the launch), 512 4.1, 2,047 6.2, 8,192 10.8
-// (8.9 MB: 0.8 TB/s); every score in 64 bits 24 us, neighbours left to route_exact 14.5.
+// What bounds it: latency.  A token is a chain of `top` + 2 reductions and the groups' ranks, some 40 dependent shuffles, on one warp; 64 registers
+// let an SM hold 32 of them, so that 8,192 tokens are 1.7 rounds, and the issue slots are half full (52 %).  Sigmoid scores with a correction, 8 of
+// 256 experts in 8 groups: 61 tokens 3.2 us (2.3 of them the launch), 512 3.8, 2,047 6.0, 8,192 10.8 (8.9 MB: 0.8 TB/s); every score in
+// 64 bits 24 us, neighbours left to route_exact 14.5.
 #include "common.cuh"
 
 namespace iian {
