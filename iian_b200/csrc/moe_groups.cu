@@ -11,7 +11,7 @@
 // weighs 0 (a softmax over logits of minus infinity alone is such a row).
 //
 // What bounds it: latency.  A token is a chain of `top` + 2 reductions and the groups' ranks, some 40 dependent shuffles, on one warp; 64 registers
-// let an SM hold 32 of them, so that 8,192 tokens are 1.7 rounds, and the issue slots are half full (52 %).  Sigmoid scores with a correction, 8 of
+// let an SM hold 32 of them, so that 8,192 tokens are 1.7 waves, and the issue slots are half full (52 %).  Sigmoid scores with a correction, 8 of
 // 256 experts in 8 groups: 61 tokens 3.2 us (2.3 of them the launch), 512 3.8, 2,047 6.0, 8,192 10.8 (8.9 MB: 0.8 TB/s); every score in
 // 64 bits 24 us, neighbours left to route_exact 14.5.
 #include "common.cuh"
