@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(128) moe_route_grouped_kernel(const RouteArgs 
         // (the two that a group's score is made of may lie further from 0 than it does)
         const float widest = two ? fmaxf(fabsf(number(k1)), fabsf(number(k2))) : fabsf(gs);
         const bool border = live && !(lo - hi > 2.0f * near_of(widest));
-        unsure = live && !(widest < 1e30f);
+        // (an infinity whose key holds a slot's number in its place is no number, which a maximum passes over: each by itself)
+        unsure = live && !(fabsf(number(k1)) < 1e30f && (!two || fabsf(number(k2)) < 1e30f));
         if (__any_sync(0xffffffffu, border)) {
             // the groups again by the scores in 64 bits of each lane's two largest, where it is certain which these are
             if constexpr (SORT && SLOTS > 2) {
